@@ -583,6 +583,91 @@ int salt_b200_q4_expert_chain_static(const void *d_gate_vals, const void *d_gate
                                      const void *d_down_biases, int hidden, int inter, const float *d_x,
                                      int ntok, float *d_y, void *stream);
 
+/* ---- Experts without a stack -------------------------------------------------------------------------------------- */
+/* Operators on device pointers for a host that keeps its own layers: routing with scores, balance bias and expert groups,
+ * MXFP4 (W4A4) quantisation and products, and the weighted combine.  No counterpart in the reference (its router is the
+ * softmax top-k of models/gemma4-26b-a4b/src/gemma4.c:132-186, its four-bit formats are affine Q4 and NVFP4).
+ *
+ *   salt_b200_route_experts -> salt_b200_mxfp4_quantize (token rows in grouped order) -> salt_b200_mxfp4_experts (gate | up)
+ *   -> salt_b200_mxfp4_quantize -> salt_b200_mxfp4_experts (down) -> salt_b200_combine_experts
+ *
+ * Every call is asynchronous on `stream` (a cudaStream_t, NULL = default stream), keeps nothing between calls, allocates
+ * nothing and may be captured; only weights_create / _destroy / _status allocate or synchronise.  All pointers are memory of the
+ * current device unless stated; strides count elements.  0 = accepted, -1 = refused before anything was launched.  One
+ * calling thread at a time. */
+#define SALT_B200_F32 0
+#define SALT_B200_BF16 1
+#define SALT_B200_F16 2
+
+#define SALT_B200_SCORE_SOFTMAX 0
+#define SALT_B200_SCORE_SIGMOID 1
+/* scores: softmax over the row, or 1 / (1 + exp(-logit)).  key = score + bias[e] (without a bias the logits order the
+ * experts).  The n_experts fall into n_groups (1 to 32, a divisor) of consecutive experts; a group's score is the sum of its best
+ * group_top (1 or 2) keys, the topk_groups best groups stay, and the topk (at most 32) best keys of their experts are selected;
+ * the lowest index wins a tie.  weight = scale * score, divided by the sum of the selected scores if renormalize (a sum of zero
+ * in double leaves zeros).  The bias never enters a weight.  The selection is that of 64-bit scores, whatever the type of the logits.
+ * An expert whose logit or key is NaN or -infinity is never selected and takes no part in the softmax; logits of +infinity share
+ * the whole softmax.  n_experts is at most 1024. */
+typedef struct SaltB200RouteSpec {
+    int n_experts, topk, scoring, n_groups, topk_groups, group_top, renormalize;
+    float scale;
+} SaltB200RouteSpec;
+/* d_logits [rows][row_stride] of `dtype`; d_bias [n_experts] or NULL -> d_selected, d_weights [rows][topk], experts ascending
+ * within a token; where fewer than topk can be selected the last places hold -1 and 0.  The grouping (all three or none, as
+ * reference src/tensorops.c:239-289): d_group_offsets [n_experts + 1], d_grouped_to_canonical and d_canonical_to_grouped
+ * [rows * topk]; a place of -1 belongs to no group (its d_canonical_to_grouped is -1, and so are the entries of
+ * d_grouped_to_canonical behind the last group).  rows * topk is at most 2^24; no rows leave all groups empty. */
+int salt_b200_route_experts(const SaltB200RouteSpec *spec, const void *d_logits, int dtype, size_t row_stride, int rows,
+                            const float *d_bias, int32_t *d_selected, float *d_weights, int32_t *d_group_offsets,
+                            int32_t *d_grouped_to_canonical, int32_t *d_canonical_to_grouped, void *stream);
+
+/* MXFP4: per 32 columns one E8M0 scale byte (2^(byte - 127), 255 = NaN) and 32 E2M1 codes, two per byte, even column low.
+ * Quantisation: byte = floor(log2(largest magnitude)) - 2 + 127, at least 0; codes to the nearest, ties to the even code, magnitudes
+ * beyond 6 units become 6; a block that holds a NaN or an infinity becomes NaN.  cols is a multiple of 32, at most
+ * SALT_B200_MXFP4_MAX_COLS.
+ * Row i of the result is row d_row_index[i] / index_div of d_x [src_rows][row_stride] (with d_grouped_to_canonical and topk: the
+ * token rows in grouped order), or row i when d_row_index is NULL (index_div is not read then); an index below zero or beyond
+ * src_rows leaves the row's outputs as they were.  d_codes [rows][cols / 2], d_scales [rows][salt_b200_mxfp4_scale_pitch(cols)] (the
+ * bytes behind cols / 32 are not written, nor read by the products), d_values [rows][cols] of `dtype` or NULL: what the codes
+ * stand for.  d_x, its rows, and the outputs begin on 16 bytes. */
+#define SALT_B200_MXFP4_MAX_COLS 131072
+size_t salt_b200_mxfp4_scale_pitch(int cols);
+int salt_b200_mxfp4_quantize(const void *d_x, int dtype, size_t row_stride, int src_rows, int cols, const int32_t *d_row_index,
+                             int index_div, int rows, uint8_t *d_codes, uint8_t *d_scales, void *d_values, void *stream);
+
+#define SALT_B200_ACT_NONE 0
+#define SALT_B200_ACT_GELU_TANH 1
+#define SALT_B200_ACT_SILU 2
+/* Matrices [rows][cols] of n_experts experts (1: a dense projection).  Pointers are HOST or device memory; they are read on
+ * `stream` before create returns and not kept: the handle holds its own copy, laid out once for the kernels.  codes
+ * [n_experts][rows][cols / 2], scales [n_experts][rows][cols / 32]; strides in bytes, 0 = dense.  With up_codes and up_scales (same
+ * strides) the pair is gated: a product returns activation(gate row) * up row, and activation must be one of the two
+ * functions.  A handle belongs to the device that is current when it is made; calls on another device are refused. */
+typedef struct SaltB200Mxfp4Spec {
+    int rows, cols, n_experts, activation;
+    const void *codes, *scales, *up_codes, *up_scales;
+    size_t expert_code_stride, expert_scale_stride, scale_row_stride;
+} SaltB200Mxfp4Spec;
+int salt_b200_mxfp4_weights_create(const SaltB200Mxfp4Spec *spec, void *stream, void **weights_out);
+int salt_b200_mxfp4_weights_destroy(void *weights);      /* after every call that uses it has finished */
+/* y[i] = W x_i for `rows` quantised rows; n_experts must be 1.  d_y [rows][y_row_stride] of y_dtype.  Sums in 32 bits, rounded once.
+ * A block's scale product and sum must lie within the range of 32 bits. */
+int salt_b200_mxfp4_matmul(void *weights, const uint8_t *d_codes, const uint8_t *d_scales, int rows, void *d_y, int y_dtype,
+                           size_t y_row_stride, void *stream);
+/* The same with row i multiplied by the matrix of its group: rows d_group_offsets[e] .. d_group_offsets[e + 1] (ascending) are
+ * those of expert e; rows in no group keep what d_y held.  `rows` bounds the rows that are read and written. */
+int salt_b200_mxfp4_experts(void *weights, const uint8_t *d_codes, const uint8_t *d_scales, const int32_t *d_group_offsets,
+                            int rows, void *d_y, int y_dtype, size_t y_row_stride, void *stream);
+/* Synchronise `stream`, read and clear the handle's device error word.  0 = clean, -1 = refused or failed. */
+int salt_b200_mxfp4_status(void *weights, void *stream);
+
+/* d_y[t] = sum over j of d_weights[t * topk + j] * d_rows[d_row_index[t * topk + j]], j ascending, in 32 bits, rounded once;
+ * d_row_index NULL: row t * topk + j.  An index below zero or beyond n_rows adds nothing; a weight of zero still multiplies its row.
+ * topk is at most 32.  Any alignment of whole elements. */
+int salt_b200_combine_experts(const void *d_rows, int dtype, size_t row_stride, int n_rows, int cols, const int32_t *d_row_index,
+                              const float *d_weights, int tokens, int topk, void *d_y, int y_dtype, size_t y_row_stride,
+                              void *stream);
+
 #ifdef __cplusplus
 }
 #endif

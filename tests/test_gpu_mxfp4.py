@@ -1,0 +1,329 @@
+"""MXFP4 quantisation (codes and scales equal, bit for bit) and products (within the rounding of 32-bit sums) against the statement
+in 64 bits."""
+import importlib
+
+import numpy as np
+import pytest
+
+import expert_ops_oracle as eo
+
+pytestmark = pytest.mark.gpu
+ex = importlib.import_module("salt-core_b200.experts")
+TYPES = {"f32": "float32", "bf16": "bfloat16", "f16": "float16"}
+
+
+def tt(name):
+    import torch
+    return getattr(torch, TYPES[name])
+
+
+def quantize(x, dtype, index=None, div=1, rows=None, values=True, pad=0):
+    """x: torch [n][cols] -> (codes packed, scales, values), the rows and bytes that are not written left at 0x5a."""
+    import torch
+    n, cols = x.shape
+    held = torch.zeros(n, cols + pad, dtype=x.dtype, device="cuda")
+    held[:, :cols] = x
+    rows = n if rows is None else rows
+    codes = torch.full((rows + 2, cols // 2), 0x5a, dtype=torch.uint8, device="cuda")
+    scales = torch.full((rows + 2, eo.scale_pitch(cols)), 0x5a, dtype=torch.uint8, device="cuda")
+    vals = torch.full((rows + 2, cols), 55.0, dtype=x.dtype, device="cuda")
+    torch.cuda.synchronize()
+    assert ex.quantize(held.data_ptr(), n, cols, codes.data_ptr(), scales.data_ptr(), dtype=dtype, row_stride=cols + pad, rows=rows,
+                       d_row_index=0 if index is None else index.data_ptr(), index_div=div,
+                       d_values=vals.data_ptr() if values else 0) == 0
+    torch.cuda.synchronize()
+    return codes, scales, vals
+
+
+def check_quantize(x, dtype, **k):
+    import torch
+    codes, scales, vals = quantize(x, dtype, **k)
+    n, cols = x.shape
+    code, byte = eo.mx_quantize(x.double().cpu().numpy())
+    nb = cols // 32
+    assert np.array_equal(scales[:n, :nb].cpu().numpy(), byte)
+    assert np.array_equal(codes[:n].cpu().numpy(), eo.mx_pack(code))
+    assert (scales[:, nb:] == 0x5a).all() and (scales[n:] == 0x5a).all() and (codes[n:] == 0x5a).all()
+    want = torch.from_numpy(eo.mx_values(code, byte)).to(x.dtype).cuda()
+    assert torch.equal(torch.nan_to_num(vals[:n], nan=77.0), torch.nan_to_num(want, nan=77.0)) and (vals[n:] == 55.0).all()
+    assert torch.equal(torch.isnan(vals[:n]), torch.isnan(want))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,cols,pad", [(1, 32, 0), (3, 64, 8), (17, 96, 0), (5, 1056, 16), (130, 2816, 0), (2, 5120, 0)])
+def test_quantize(dtype, n, cols, pad):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(n + cols)
+    x = torch.randn(n, cols, device="cuda", generator=g) * torch.exp2(6 * torch.randn(n, cols, device="cuda", generator=g).clamp(-2, 1.5))
+    check_quantize(x.to(tt(dtype)), dtype, pad=pad)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_quantize_every_tie_and_extreme(dtype):
+    """All halfway values at many scales, both signs; zeros; subnormals; the largest finite value; infinities and NaN."""
+    import torch
+    t = tt(dtype)
+    info = torch.finfo(t)
+    ties = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 7.75, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0]).repeat(2)
+    ties[16:] *= -1
+    ties[15] = 4.0
+    rows = [ties * 2.0 ** e for e in (range(-9, 13) if dtype == "f16" else range(-120, 125, 7))]
+    zero = torch.zeros(32)
+    zero[::2] = -0.0
+    rows += [zero, torch.full((32,), info.max), torch.full((32,), info.tiny), torch.full((32,), info.smallest_normal / 4)]
+    rows.append(torch.linspace(-1, 1, 32) * info.tiny)
+    for bad in (torch.nan, torch.inf, -torch.inf):
+        r = torch.ones(32)
+        r[7] = bad
+        rows.append(r)
+    check_quantize(torch.stack(rows).to(t).cuda(), dtype)
+
+
+def test_quantize_by_index():
+    """Rows in grouped order, the same row several times; an index below zero or beyond the rows leaves its row alone."""
+    import torch
+    T, k, cols = 21, 4, 160
+    x = torch.randn(T, cols, device="cuda").bfloat16()
+    index = torch.randperm(T * k, device="cuda").to(torch.int32)
+    index[[0, 9, 30]] = torch.tensor([-1, T * k, -2 ** 31], dtype=torch.int32, device="cuda")
+    codes, scales, vals = quantize(x, "bf16", index, k, T * k)
+    code, byte = eo.mx_quantize(x.double().cpu().numpy())
+    for i, at in enumerate(index.tolist()):
+        if 0 <= at < T * k:
+            assert np.array_equal(codes[i].cpu().numpy(), eo.mx_pack(code[at // k])), i
+            assert np.array_equal(scales[i, :5].cpu().numpy(), byte[at // k]), i
+        else:
+            assert (codes[i] == 0x5a).all() and (scales[i] == 0x5a).all() and (vals[i] == 55.0).all()
+    assert (codes[T * k:] == 0x5a).all()
+    again = quantize(x, "bf16", index, k, T * k, values=False)
+    assert torch.equal(again[0], codes) and torch.equal(again[1], scales) and (again[2] == 55.0).all()
+
+
+def weights(rng, *shape):
+    """Random matrices as codes and scale bytes [..., rows, cols], every code among them, scales over a few binades."""
+    code = rng.integers(0, 16, shape).astype(np.uint8)
+    byte = rng.integers(118, 127, (*shape[:-1], shape[-1] // 32)).astype(np.uint8)
+    return code, byte
+
+
+def device(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+class Held:
+    """A handle and the values its matrices stand for."""
+
+    def __init__(self, seed, E, R, C, activation=None, host=False):
+        rng = np.random.default_rng(seed)
+        self.parts = [weights(rng, E, R, C) for _ in range(2 if activation else 1)]
+        packed = [(eo.mx_pack(c), b) for c, b in self.parts]
+        if not host:
+            packed = [(device(c), device(b)) for c, b in packed]
+        addr = [a.ctypes.data if host else a.data_ptr() for p in packed for a in p]
+        self.activation = activation
+        self.handle = ex.Mxfp4Weights(R, C, E, *addr[:2], **(dict(up_codes=addr[2], up_scales=addr[3], activation=activation)
+                                                             if activation else {}))
+        self.values = [eo.mx_values(c, b) for c, b in self.parts]
+
+    def want(self, xv, e=0):
+        if self.activation:
+            return eo.gated(self.activation, xv, self.values[0][e], self.values[1][e])
+        return eo.product(xv, self.values[0][e])
+
+
+def acts(seed, n, C, dtype="f32"):
+    """Quantised rows on the device and the values they stand for."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(max(n, 1), C, device="cuda", generator=g).to(tt(dtype))[:n]
+    codes, scales, _ = quantize(x, dtype)
+    code, byte = eo.mx_quantize(x.double().cpu().numpy()) if n else (np.zeros((0, C), np.uint8), np.zeros((0, C // 32), np.uint8))
+    return codes, scales, eo.mx_values(code, byte)
+
+
+def check_matmul(held, n, R, C, y_dtype="f32", y_pad=0, seed=0):
+    import torch
+    codes, scales, xv = acts(seed + n, n, C)
+    y = torch.full((n + 1, R + y_pad), 55.0, dtype=tt(y_dtype), device="cuda")
+    torch.cuda.synchronize()
+    assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr(), y_dtype=y_dtype, y_row_stride=R + y_pad) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    want, err = held.want(xv)
+    eo.close(y[:n, :R].double().cpu().numpy(), want, err, y_dtype, f"{n} rows of {R} x {C}")
+    assert (y[n:] == 55.0).all() and (y[:, R:] == 55.0).all()
+
+
+SHAPES = [(1, 32), (7, 64), (64, 96), (129, 288), (128, 256), (300, 1056), (704, 2816), (257, 544)]
+
+
+@pytest.mark.parametrize("R,C", SHAPES)
+@pytest.mark.parametrize("activation", [None, "silu", "gelu_tanh"])
+def test_matmul_shapes(R, C, activation):
+    held = Held(R + C, 1, R, C, activation)
+    for n in (1, 2, 3, 5, 8, 9, 16, 17, 33, 64, 65, 129, 300):
+        check_matmul(held, n, R, C, seed=R)
+
+
+@pytest.mark.parametrize("y_dtype", list(TYPES))
+@pytest.mark.parametrize("y_pad", [0, 1, 8])
+@pytest.mark.parametrize("activation", [None, "silu"])
+def test_matmul_results(y_dtype, y_pad, activation):
+    held = Held(11, 1, 203, 320, activation, host=True)
+    for n in (1, 4, 50, 140):
+        check_matmul(held, n, 203, 320, y_dtype, y_pad)
+
+
+def test_wide_rows():
+    """Rows at the documented limit, and one that leaves room for fewer tokens a pass."""
+    for C in (131072, 40960):
+        held = Held(C, 1, 40, C)
+        for n in (1, 6, 20):
+            check_matmul(held, n, 40, C)
+
+
+def test_no_rows():
+    held = Held(3, 2, 32, 64)
+    assert held.handle.experts(0, 0, 0x1000, 0, 0) == 0
+    assert Held(3, 1, 32, 64).handle.matmul(0, 0, 0, 0) == 0
+
+
+def test_bad_scales_stay_where_they_are():
+    """A NaN block of an activation row or of a weight row makes the results that use it NaN, and no others."""
+    import torch
+    R, C = 70, 512
+    rng = np.random.default_rng(8)
+    code, byte = weights(rng, 1, R, C)
+    byte[0, 13, 5] = 255
+    w = [device(eo.mx_pack(code)), device(byte)]
+    handle = ex.Mxfp4Weights(R, C, 1, w[0].data_ptr(), w[1].data_ptr())
+    for n in (1, 3, 8, 40, 130):
+        x = torch.randn(n, C, device="cuda")
+        x[n // 2, 100] = torch.nan
+        codes, scales, _ = quantize(x, "f32")
+        y = torch.empty(n, R, device="cuda")
+        assert handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr()) == 0
+        nan = torch.isnan(y).cpu().numpy()
+        want = np.zeros((n, R), bool)
+        want[:, 13] = True
+        want[n // 2] = True
+        assert np.array_equal(nan, want), n
+
+
+GROUPS = {"token": [1, 0, 1, 0, 0, 1], "even": [3, 3, 3, 3, 3, 3], "one": [0, 0, 40, 0, 0, 0], "ragged": [1, 17, 0, 130, 5, 64],
+          "last": [0, 0, 0, 0, 0, 9], "large": [240, 1, 300, 225, 16, 224]}
+
+
+@pytest.mark.parametrize("name", list(GROUPS))
+@pytest.mark.parametrize("R,C,activation", [(96, 288, "silu"), (200, 512, None), (64, 96, "gelu_tanh"), (129, 1056, None)])
+def test_experts(name, R, C, activation):
+    """Groups of every size, empty ones, rows behind the last group, whose outputs stay."""
+    import torch
+    counts = GROUPS[name]
+    E, live, behind = len(counts), sum(counts), 5
+    held = Held(R + live, E, R, C, activation)
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    n = live + behind
+    codes, scales, xv = acts(live, n, C, "bf16")
+    off = device(offsets)
+    y = torch.full((n, R), 55.0, device="cuda")
+    torch.cuda.synchronize()
+    assert held.handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), n, y.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    got = y.double().cpu().numpy()
+    for e in range(E):
+        b, t = offsets[e], offsets[e + 1]
+        if t > b:
+            want, err = held.want(xv[b:t], e)
+            eo.close(got[b:t], want, err, "f32", f"expert {e}")
+    assert (got[live:] == 55.0).all()
+
+
+def test_many_experts():
+    """1024 experts, most of them empty."""
+    import torch
+    E, R, C = 1024, 32, 64
+    held = Held(77, E, R, C)
+    counts = np.zeros(E, np.int64)
+    counts[[0, 5, 500, 1022, 1023]] = [2, 1, 30, 3, 9]
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    n = int(counts.sum())
+    codes, scales, xv = acts(4, n, C)
+    off, y = device(offsets), torch.zeros(n, R, device="cuda")
+    torch.cuda.synchronize()
+    assert held.handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), n, y.data_ptr()) == 0
+    got = y.double().cpu().numpy()
+    for e in np.nonzero(counts)[0]:
+        want, err = held.want(xv[offsets[e]:offsets[e + 1]], e)
+        eo.close(got[offsets[e]:offsets[e + 1]], want, err, "f32", f"expert {e}")
+
+
+def test_strided_weights():
+    """Experts laid out as slots of gate codes | gate scales | up codes | up scales, scale rows further apart than they are long."""
+    import torch
+    E, R, C, pitch = 3, 40, 96, 7
+    rng = np.random.default_rng(2)
+    parts = [weights(rng, E, R, C) for _ in range(2)]
+    slot = 2 * (R * C // 2 + R * pitch) + 13
+    pool = np.zeros((E, slot), np.uint8)
+    for e in range(E):
+        at = 0
+        for code, byte in parts:
+            pool[e, at:at + R * C // 2] = eo.mx_pack(code[e]).reshape(-1)
+            at += R * C // 2
+            rows = np.full((R, pitch), 0xff, np.uint8)
+            rows[:, :C // 32] = byte[e]
+            pool[e, at:at + R * pitch] = rows.reshape(-1)
+            at += R * pitch
+    d, half = device(pool), R * C // 2 + R * pitch
+    base = d.data_ptr()
+    handle = ex.Mxfp4Weights(R, C, E, base, base + R * C // 2, up_codes=base + half, up_scales=base + half + R * C // 2, activation="silu",
+                             expert_code_stride=slot, expert_scale_stride=slot, scale_row_stride=pitch)
+    off = device(np.array([0, 2, 5, 6], np.int32))
+    codes, scales, xv = acts(1, 6, C)
+    y = torch.zeros(6, R, device="cuda")
+    torch.cuda.synchronize()
+    assert handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), 6, y.data_ptr()) == 0
+    got = y.double().cpu().numpy()
+    for e, (b, t) in enumerate(((0, 2), (2, 5), (5, 6))):
+        want, err = eo.gated("silu", xv[b:t], *[eo.mx_values(c[e], s[e]) for c, s in parts])
+        eo.close(got[b:t], want, err, "f32")
+
+
+def test_refusals_with_a_handle():
+    held = Held(1, 2, 32, 64)
+    h, P = held.handle, 0x1000
+    assert h.matmul(P, P, 1, P) == -1                    # two experts: not one matrix
+    assert h.experts(P, P, 0, 1, P) == -1
+    for bad in (dict(d_codes=0), dict(d_scales=0), dict(d_y=0), dict(rows=-1), dict(d_codes=P + 8), dict(d_scales=P + 1), dict(d_y=P + 2),
+                dict(y_row_stride=31)):
+        assert h.experts(**{**dict(d_codes=P, d_scales=P, d_group_offsets=P, rows=1, d_y=P), **bad}) == -1, bad
+    assert h.lib.salt_b200_mxfp4_experts(h.handle, P, P, P, 1, P, 3, 32, 0) == -1
+
+
+@pytest.mark.parametrize("n", [1, 7, 90, 400])
+def test_repeated_and_captured(n):
+    """The same bits again, on another stream, and replayed from a graph on new activations."""
+    import torch
+    R, C = 300, 1056
+    held = Held(6, 1, R, C)
+    codes, scales, xv = acts(5, n, C)
+    y, z = torch.empty(n, R, device="cuda"), torch.empty(n, R, device="cuda")
+    torch.cuda.synchronize()
+    assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr()) == 0
+    s = torch.cuda.Stream()
+    assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, z.data_ptr(), stream=s.cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, z.data_ptr(), stream=torch.cuda.current_stream().cuda_stream) == 0
+    new = acts(6, n, C)
+    codes.copy_(new[0])
+    scales.copy_(new[1])
+    g.replay()
+    torch.cuda.synchronize()
+    want, err = held.want(new[2])
+    eo.close(z.double().cpu().numpy(), want, err, "f32")
