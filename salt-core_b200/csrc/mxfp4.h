@@ -20,6 +20,7 @@ struct Mxfp4Weights {
     uint8_t* scales;
     int* status;
 };
+struct Mxfp4Handle : Mxfp4Weights { CUtensorMap map; };
 
 struct Mxfp4Call {
     const uint8_t* codes;        // [rows][cols / 2]
@@ -33,6 +34,10 @@ struct Mxfp4Call {
 
 // mxfp4_few_rows.cu: passes of up to eight rows, exact integer sums per block
 cudaError_t launch_mxfp4_few_rows(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
+
+// mxfp4_tensor.cu: block-scaled tensor-core products
+cudaError_t make_mxfp4_weight_map(CUtensorMap* out, const Mxfp4Weights& w);
+cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const CUtensorMap& weight_map, const Mxfp4Call& c, cudaStream_t stream);
 
 // y = act(gate) * up
 __device__ __forceinline__ float gate_act(int activation, float g) {

@@ -1,0 +1,419 @@
+// MXFP4 products on the tensor cores: block-scaled tcgen05.mma.kind::mxf4 (E2M1 codes in both operands, one E8M0 scale per 32
+// columns of each, 32-bit accumulation in TMEM), dense or by expert groups.
+//
+// A unit = 128 stored weight rows (M) times one pass of a group's rows (N, a multiple of 16), K in chunks of 256 columns = one
+// 128-byte row of packed codes = four MMAs of K = 64.  Persistent blocks, one per SM; unit u of the launch goes to block u mod
+// grid, a group's row tiles next to one another, so the blocks that work at the same time read the same activations.  Which
+// group a unit belongs to is found in a prefix table over the groups' passes, made by every block from the device offsets.
+// Warp roles:
+//   warp 9      producer: TMA copies of the weight codes (3-D map: byte column, row, expert), of the rows' codes (boxes of 32 rows)
+//               and of the weights' scale tiles, which lie in memory as the tensor core reads them
+//   warps 0-3   scales of the rows: 16 bytes per row and pair of chunks, loaded a pair ahead, written to shared memory in the order
+//               of a scale tile
+//   warp 8      issuer: tcgen05.cp of the chunk's scale tiles to TMEM, then its four MMAs; both run in issue order
+//   warps 4-7   epilogue: lane = weight row, column = row of the result; a gated pair's two rows are neighbouring lanes
+// Every mbarrier wait is bounded; on expiry the block raises its failure flag, sets SB_ERR_TIMEOUT, waits (bounded) for copies
+// and MMAs in flight, frees its TMEM and returns.
+#include <algorithm>
+
+#include "../../include/salt_gpu_b200.h"
+#include "float_types.cuh"
+#include "internal.h"
+#include "mxfp4.h"
+#include "pdl.cuh"
+#include "umma.cuh"
+
+namespace sb {
+namespace {
+
+constexpr int MT_THREADS = 320;          // warps 0-3 scales, 4-7 epilogue, 8 issuer, 9 producer
+constexpr int MT_CHUNK = 128;            // packed bytes of a K chunk
+constexpr int MT_A_BYTES = 128 * MT_CHUNK;
+constexpr int MT_BOX = 32;               // rows of an activation copy
+constexpr int MT_MAX_N = 224;            // two accumulators of 224 columns and 64 columns of scales fill TMEM
+constexpr uint32_t MT_TMEM_COLS = 512, MT_SF_BASE = 448, MT_SF_STRIDE = 32, MT_SFB = 8;
+constexpr int MT_SFA_BYTES = 1024, MT_SFB_BYTES = 2048;
+constexpr int MT_MAX_STAGES = 8;
+constexpr int MT_SMEM = 222 * 1024;
+
+struct MxTensorArgs {
+    Mxfp4Weights w;
+    Mxfp4Call c;
+    int cap;                             // most rows of a pass, a multiple of 16
+    int stages, stage_bytes;
+    int chunks;
+};
+
+struct MxMaps { CUtensorMap w, x; };
+
+// kind::mxf4 instruction descriptor: A = B = E2M1, K-major, E8M0 scales, `half` = which two bytes of a scale word the MMA reads.
+__device__ __forceinline__ uint32_t mx_idesc(int N, uint32_t half) {
+    return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | (1u << 27) | (half << 5) | (half << 30);
+}
+
+__device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+// 32 rows of 16 bytes, unswizzled (8-row groups 128 bytes apart), to four TMEM columns of all four lane quarters.
+__device__ __forceinline__ void scale_copy(uint32_t taddr, uint32_t smem) {
+    const uint64_t desc = make_desc((smem & 0x3ffffu) >> 4, (128u >> 4) | (1u << 14));
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+
+struct Unit { int expert, tile, row0, n, N; };   // n rows of the pass, N = n up to a multiple of 16
+
+// Passes of a group of n rows: as few as the cap allows, of equal size up to the multiple of 16.
+__device__ __forceinline__ int pass_rows(int n, int cap) {
+    const int passes = (n + cap - 1) / cap;
+    return passes ? ((n + passes - 1) / passes + 15) & ~15 : cap;
+}
+
+struct Groups {
+    const int* first;                    // [experts + 1] passes before each group (shared memory), null for one dense matrix
+    const int32_t* offsets;
+    int experts, rows, cap, tiles;
+
+    __device__ __forceinline__ bool unit(int u, Unit* out) const {
+        const int pass = u / tiles;
+        out->tile = u - pass * tiles;
+        int b = 0, t = rows, e = 0, p = pass;
+        if (first) {
+            if (pass >= first[experts]) return false;
+            int lo = 0, hi = experts;    // first[lo] <= pass < first[hi]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first[mid] <= pass) lo = mid;
+                else hi = mid;
+            }
+            e = lo;
+            p = pass - first[e];
+            b = max(offsets[e], 0);
+            t = min(offsets[e + 1], rows);
+        }
+        const int size = pass_rows(t - b, cap);
+        out->expert = e;
+        out->row0 = b + p * size;
+        out->n = min(size, t - out->row0);
+        out->N = (out->n + 15) & ~15;
+        return out->n > 0;
+    }
+};
+
+__global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTensorArgs a, const __grid_constant__ MxMaps maps) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bar_free[MT_MAX_STAGES], bar_full[MT_MAX_STAGES], bar_sf[MT_MAX_STAGES];
+    __shared__ __align__(8) uint64_t bar_done[2], bar_accfree[2], bar_drain;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_fail;
+    __shared__ int s_first[1025];
+    __shared__ int s_part[MT_THREADS / 32];
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint8_t* stage_base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    volatile int* fail = &s_fail;
+    if (tid == 0) {
+        for (int s = 0; s < a.stages; s++) {
+            mbar_init(&bar_free[s], 1);
+            mbar_init(&bar_full[s], 1);
+            mbar_init(&bar_sf[s], 4);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&bar_done[b], 1);
+            mbar_init(&bar_accfree[b], 4);
+        }
+        mbar_init(&bar_drain, 1);
+        s_fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(MT_TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    if (a.c.offsets) {
+        // passes before every group: a thread sums a run of groups, then the threads' sums are scanned
+        const int run = (a.w.experts + MT_THREADS - 1) / MT_THREADS;
+        int sum = 0;
+        for (int j = 0; j < run; j++) {
+            const int e = tid * run + j;
+            if (e >= a.w.experts) break;
+            const int n = min(a.c.offsets[e + 1], a.c.rows) - max(a.c.offsets[e], 0);
+            s_first[e] = sum;
+            if (n > 0) {
+                const int size = pass_rows(n, a.cap);
+                sum += (n + size - 1) / size;
+            }
+        }
+        int scan = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, scan, d);
+            if (lane >= d) scan += o;
+        }
+        if (lane == 31) s_part[warp] = scan;
+        __syncthreads();
+        int front = scan - sum;
+        for (int i = 0; i < warp; i++) front += s_part[i];
+        for (int j = 0; j < run; j++) {
+            const int e = tid * run + j;
+            if (e >= a.w.experts) break;
+            s_first[e] += front;
+        }
+        if (tid == MT_THREADS - 1) s_first[a.w.experts] = front + sum;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    Groups groups;
+    groups.first = a.c.offsets ? s_first : nullptr;
+    groups.offsets = a.c.offsets; groups.experts = a.w.experts; groups.rows = a.c.rows; groups.cap = a.cap; groups.tiles = a.w.row_tiles;
+    const int size = pass_rows(a.c.rows, a.cap);
+    const int units = (a.c.offsets ? s_first[a.w.experts] : (a.c.rows + size - 1) / size) * a.w.row_tiles;
+    const int b_off = MT_A_BYTES, sfa_off = a.stage_bytes - MT_SFA_BYTES - MT_SFB_BYTES, sfb_off = a.stage_bytes - MT_SFB_BYTES;
+
+    uint32_t produced = 0;
+    if (warp == 9) {
+        // ================= producer =================
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t s = 0, ph = 1;                      // a fresh barrier's previous phase counts as complete
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                Unit un;
+                if (!groups.unit(u, &un)) continue;
+                const int boxes = (un.N + MT_BOX - 1) / MT_BOX;
+                const uint32_t tx = MT_A_BYTES + MT_SFA_BYTES + boxes * (MT_BOX * MT_CHUNK);
+                const uint8_t* sfa = a.w.scales + ((size_t)un.expert * a.w.row_tiles + un.tile) * a.w.col_tiles * 512;
+                for (int kc = 0; kc < a.chunks; kc++, produced++) {
+                    if (!mbar_wait(&bar_free[s], ph, fail)) { ok = false; break; }
+                    const uint32_t dst = smem_u32(stage_base + s * a.stage_bytes);
+                    mbar_expect_tx(&bar_full[s], tx);
+                    tma_load_3d(dst, &maps.w, kc * MT_CHUNK, un.tile * 128, un.expert, &bar_full[s]);
+                    for (int b = 0; b < boxes; b++)
+                        tma_load_2d(dst + b_off + b * (MT_BOX * MT_CHUNK), &maps.x, kc * MT_CHUNK, un.row0 + b * MT_BOX, &bar_full[s]);
+                    bulk_load(dst + sfa_off, sfa + (size_t)kc * 1024, MT_SFA_BYTES, &bar_full[s]);
+                    if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 8) {
+        // ================= issuer (one thread) =================
+        // The barriers of the next stage are looked at before this stage's MMAs go out: a wait costs 150 to 250 cycles even
+        // when its phase is complete.
+        if (lane == 0) {
+            const uint32_t base = smem_u32(stage_base);
+            uint32_t s = 0, ph = 0, ready = 0, done = 0, par = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                Unit un;
+                if (!groups.unit(u, &un)) continue;
+                const uint32_t buf = done & 1u;
+                if (done >= 2u) ok = mbar_wait(&bar_accfree[buf], ((done >> 1) - 1) & 1, fail);
+                const uint32_t id0 = mx_idesc(un.N, 0), id1 = mx_idesc(un.N, 1);
+                const uint32_t d = tmem + buf * MT_MAX_N;
+                const int halves = (un.N + 127) / 128;
+                for (int kc = 0; kc < a.chunks && ok; kc++) {
+                    if (!ready) ok = mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail);
+                    if (!ok) break;
+                    uint32_t ns = s + 1, nph = ph;
+                    if (ns == (uint32_t)a.stages) { ns = 0; nph ^= 1u; }
+                    const uint32_t r_full = mbar_test(&bar_full[ns], nph), r_sf = mbar_test(&bar_sf[ns], nph);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t st = base + s * a.stage_bytes;
+                    const uint32_t sf = tmem + MT_SF_BASE + par * MT_SF_STRIDE;
+                    par ^= 1u;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        scale_copy(sf + 4 * k, st + sfa_off + k * 512);
+                        scale_copy(sf + MT_SFB + 8 * k, st + sfb_off + k * 1024);
+                        if (halves > 1) scale_copy(sf + MT_SFB + 8 * k + 4, st + sfb_off + k * 1024 + 512);
+                    }
+                    const uint32_t alo = DESC_B_LO | ((st & 0x3ffffu) >> 4), blo = alo + (b_off >> 4);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        mx_mma(d, make_desc(alo + j * 2, DESC_B_HI), make_desc(blo + j * 2, DESC_B_HI), (j & 1) ? id1 : id0,
+                               sf + 4 * (j >> 1), sf + MT_SFB + 8 * (j >> 1), (kc > 0 || j > 0) ? 1u : 0u);
+                    umma_commit(&bar_free[s]);
+                    if (kc == a.chunks - 1) umma_commit(&bar_done[buf]);
+                    ready = r_full & r_sf;
+                    s = ns;
+                    ph = nph;
+                }
+                done++;
+            }
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        // ================= scales of the rows =================
+        const int blocks = a.w.cols / 32;
+        const size_t pitch = ((size_t)blocks + 15) / 16 * 16;
+        uint32_t s = 0, ph = 1;
+        bool ok = true;
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            Unit un;
+            if (!groups.unit(u, &un)) continue;
+            const int r0 = tid, r1 = tid + 128;
+            const bool have0 = r0 < un.n, have1 = r1 < un.n;
+            const uint4 one = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+            const uint4* p0 = (const uint4*)(a.c.scales + (size_t)(un.row0 + (have0 ? r0 : 0)) * pitch);
+            const uint4* p1 = (const uint4*)(a.c.scales + (size_t)(un.row0 + (have1 ? r1 : 0)) * pitch);
+            uint4 n0 = have0 ? p0[0] : one, n1 = have1 ? p1[0] : one, c0 = n0, c1 = n1;
+            const uint32_t at0 = (r0 & 31) * 16 + (r0 >> 5) * 4;     // r1: the same in the second 512 bytes
+            for (int kc = 0; kc < a.chunks && ok; kc++) {
+                if (!(kc & 1)) {
+                    c0 = n0;
+                    c1 = n1;
+                    if (kc + 2 < a.chunks) {
+                        if (have0) n0 = p0[(kc >> 1) + 1];
+                        if (have1) n1 = p1[(kc >> 1) + 1];
+                    }
+                }
+                uint32_t w[4] = {(kc & 1) ? c0.z : c0.x, (kc & 1) ? c0.w : c0.y, (kc & 1) ? c1.z : c1.x, (kc & 1) ? c1.w : c1.y};
+                if (kc * 8 + 8 > blocks) {               // blocks behind the last column read as 2^0
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        const int left = blocks - kc * 8 - i * 4;
+                        const uint32_t keep = left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1u : 0u;
+                        w[i] = (w[i] & keep) | (0x7f7f7f7fu & ~keep);
+                        w[2 + i] = (w[2 + i] & keep) | (0x7f7f7f7fu & ~keep);
+                    }
+                }
+                if (lane == 0) ok = mbar_wait(&bar_free[s], ph, fail);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                if (ok) {
+                    uint8_t* sfb = stage_base + s * a.stage_bytes + sfb_off;
+                    *(uint32_t*)(sfb + at0) = w[0];
+                    *(uint32_t*)(sfb + 1024 + at0) = w[1];
+                    if (un.N > 128) {
+                        *(uint32_t*)(sfb + 512 + at0) = w[2];
+                        *(uint32_t*)(sfb + 1536 + at0) = w[3];
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_sf[s]);  // always: the issuer never waits for a warp that gave up
+                if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else {
+        // ================= epilogue (TMEM lane quarter warp - 4) =================
+        const int q = warp - 4;
+        const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
+        uint32_t done = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            Unit un;
+            if (!groups.unit(u, &un)) continue;
+            const int m = un.tile * 128 + q * 32 + lane;
+            const bool live = m < a.w.stored_rows;
+            const uint32_t buf = done & 1u;
+            ok = mbar_wait(&bar_done[buf], (done >> 1) & 1, fail);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for (int n0 = 0; n0 < un.N; n0 += 32) {
+                uint32_t acc[32];
+                tmem_ld32(trow + buf * MT_MAX_N + n0, acc);
+                const size_t row = (size_t)(un.row0 + n0);
+                if (a.w.activation) {
+                    // lanes 2 i and 2 i + 1 hold gate and up of the same result: the even lane takes even rows, the odd lane odd ones
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float mine = __uint_as_float((lane & 1) ? acc[k + 1] : acc[k]);
+                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float((lane & 1) ? acc[k] : acc[k + 1]), 1);
+                        const int n = n0 + k + (lane & 1);
+                        const float v = (lane & 1) ? gate_act(a.w.activation, other) * mine : gate_act(a.w.activation, mine) * other;
+                        if (live && n < un.n) store_float(a.c.y, a.c.y_type, (row + k + (lane & 1)) * a.c.y_stride + (m >> 1), v);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        if (live && n0 + k < un.n) store_float(a.c.y, a.c.y_type, (row + k) * a.c.y_stride + m, __uint_as_float(acc[k]));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_accfree[buf]);
+            done++;
+        }
+    }
+
+    __syncthreads();
+    if (*fail) {
+        if (tid == 0) atomicOr(a.w.status, SB_ERR_TIMEOUT);
+        // wait (bounded, no early exit) for the copies requested and the MMAs issued before TMEM and shared memory are released
+        if (warp == 9 && lane == 0) {
+            int none = 0;
+            const uint32_t n = (uint32_t)a.stages;
+            for (uint32_t t = produced > n ? produced - n : 0; t < produced; t++) (void)mbar_wait(&bar_full[t % n], (t / n) & 1, &none);
+        }
+        __syncthreads();
+        if (warp == 8 && lane == 0) {
+            int none = 0;
+            umma_commit(&bar_drain);
+            (void)mbar_wait(&bar_drain, 0, &none);
+        }
+        __syncthreads();
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(MT_TMEM_COLS) : "memory");
+}
+
+}  // namespace
+
+cudaError_t make_mxfp4_weight_map(CUtensorMap* out, const Mxfp4Weights& w) {
+    TensorMapEncodeFn encode = nullptr;
+    const cudaError_t e = tensor_map_encoder(&encode);
+    if (e != cudaSuccess) return e;
+    const cuuint64_t row = (cuuint64_t)w.cols / 2;
+    cuuint64_t dims[3] = {row, (cuuint64_t)w.stored_rows, (cuuint64_t)w.experts};
+    cuuint64_t strides[2] = {row, row * w.stored_rows};
+    cuuint32_t box[3] = {(cuuint32_t)MT_CHUNK, 128u, 1u}, estr[3] = {1, 1, 1};
+    return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w.codes, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? cudaSuccess
+               : cudaErrorInvalidValue;
+}
+
+cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const CUtensorMap& weight_map, const Mxfp4Call& c, cudaStream_t stream) {
+    TensorMapEncodeFn encode = nullptr;
+    cudaError_t e = tensor_map_encoder(&encode);
+    if (e != cudaSuccess) return e;
+    MxMaps maps;
+    maps.w = weight_map;
+    cuuint64_t dims[2] = {(cuuint64_t)w.cols / 2, (cuuint64_t)c.rows}, strides[1] = {(cuuint64_t)w.cols / 2};
+    cuuint32_t box[2] = {(cuuint32_t)MT_CHUNK, (cuuint32_t)MT_BOX}, estr[2] = {1, 1};
+    if (encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(c.codes), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return cudaErrorInvalidValue;
+    MxTensorArgs a;
+    a.w = w;
+    a.c = c;
+    a.cap = MT_MAX_N;
+    a.chunks = (w.cols + 255) / 256;
+    a.stage_bytes = MT_A_BYTES + a.cap * MT_CHUNK + MT_SFA_BYTES + MT_SFB_BYTES;
+    a.stages = std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes);
+    const size_t smem = (size_t)a.stages * a.stage_bytes + 1024;
+    if ((e = ensure_dynamic_smem((const void*)mxfp4_tensor_kernel, smem)) != cudaSuccess) return e;
+    const long long passes = c.offsets ? (long long)c.rows / a.cap + std::min(c.rows, w.experts) + 1 : (c.rows + a.cap - 1) / a.cap + 1;
+    const int grid = (int)std::min<long long>(device_sms(), passes * w.row_tiles);
+    return launch_pdl(mxfp4_tensor_kernel, dim3(grid), dim3(MT_THREADS), smem, stream, a, maps);
+}
+
+}  // namespace sb

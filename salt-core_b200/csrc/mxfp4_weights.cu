@@ -32,7 +32,7 @@ bool on_device(const Mxfp4Weights* w) {
     return cuda_ok(cudaGetDevice(&dev), "device") && dev == w->device;
 }
 
-void free_weights(Mxfp4Weights* w) {
+void free_weights(Mxfp4Handle* w) {
     if (w->codes) cudaFree(w->codes);
     if (w->scales) cudaFree(w->scales);
     if (w->status) cudaFree(w->status);
@@ -67,14 +67,15 @@ bool upload(const SaltB200Mxfp4Spec& s, Mxfp4Weights* w, uint8_t* staged, cudaSt
     return cuda_ok(cudaStreamSynchronize(stream), "mxfp4 upload");
 }
 
-int product(Mxfp4Weights* w, const uint8_t* codes, const uint8_t* scales, const int32_t* offsets, int rows, void* y, int y_type,
+int product(Mxfp4Handle* w, const uint8_t* codes, const uint8_t* scales, const int32_t* offsets, int rows, void* y, int y_type,
             size_t y_stride, cudaStream_t stream) {
     if (!w || !on_device(w) || rows < 0 || !float_type_ok(y_type) || y_stride < (size_t)w->rows || y_stride > (size_t)1 << 40) return -1;
     if (rows == 0) return 0;
     if (!codes || !scales || !y || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)y % float_type_size(y_type)) return -1;
     Mxfp4Call c;
     c.codes = codes; c.scales = scales; c.offsets = offsets; c.rows = rows; c.y = y; c.y_type = y_type; c.y_stride = y_stride;
-    return cuda_ok(launch_mxfp4_few_rows(*w, c, stream), "mxfp4 product") ? 0 : -1;
+    const bool few = rows <= (offsets ? 2 * w->experts : 8);
+    return cuda_ok(few ? launch_mxfp4_few_rows(*w, c, stream) : launch_mxfp4_tensor(*w, w->map, c, stream), "mxfp4 product") ? 0 : -1;
 }
 
 }  // namespace
@@ -100,7 +101,7 @@ int salt_b200_mxfp4_weights_create(const SaltB200Mxfp4Spec* spec, void* stream, 
     if (!cuda_ok(cudaGetDeviceCount(&ndev), "device count") || ndev < 1 || !cuda_ok(cudaGetDevice(&dev), "device") ||
         !cuda_ok(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev), "capability") || major != 10)
         return -1;
-    Mxfp4Weights* w = new (std::nothrow) Mxfp4Weights();
+    Mxfp4Handle* w = new (std::nothrow) Mxfp4Handle();
     if (!w) return -1;
     w->device = dev; w->rows = s.rows; w->cols = s.cols; w->experts = s.n_experts;
     w->stored_rows = gated ? 2 * s.rows : s.rows;
@@ -114,7 +115,7 @@ int salt_b200_mxfp4_weights_create(const SaltB200Mxfp4Spec* spec, void* stream, 
               cuda_ok(cudaMalloc((void**)&w->status, sizeof(int)), "mxfp4 status") &&
               cuda_ok(cudaMalloc((void**)&staged, (size_t)w->stored_rows * (s.cols / 32)), "mxfp4 staging") &&
               cuda_ok(cudaMemsetAsync(w->status, 0, sizeof(int), (cudaStream_t)stream), "mxfp4 status") &&
-              upload(s, w, staged, (cudaStream_t)stream);
+              upload(s, w, staged, (cudaStream_t)stream) && cuda_ok(make_mxfp4_weight_map(&w->map, *w), "mxfp4 map");
     if (staged) cudaFree(staged);
     if (!ok) {
         free_weights(w);
@@ -126,13 +127,13 @@ int salt_b200_mxfp4_weights_create(const SaltB200Mxfp4Spec* spec, void* stream, 
 
 int salt_b200_mxfp4_weights_destroy(void* weights) {
     if (!weights) return -1;
-    sb::free_weights((sb::Mxfp4Weights*)weights);
+    sb::free_weights((sb::Mxfp4Handle*)weights);
     return 0;
 }
 
 int salt_b200_mxfp4_matmul(void* weights, const uint8_t* d_codes, const uint8_t* d_scales, int rows, void* d_y, int y_dtype,
                            size_t y_row_stride, void* stream) {
-    sb::Mxfp4Weights* w = (sb::Mxfp4Weights*)weights;
+    sb::Mxfp4Handle* w = (sb::Mxfp4Handle*)weights;
     if (!w || w->experts != 1) return -1;
     return sb::product(w, d_codes, d_scales, nullptr, rows, d_y, y_dtype, y_row_stride, (cudaStream_t)stream);
 }
@@ -140,13 +141,13 @@ int salt_b200_mxfp4_matmul(void* weights, const uint8_t* d_codes, const uint8_t*
 int salt_b200_mxfp4_experts(void* weights, const uint8_t* d_codes, const uint8_t* d_scales, const int32_t* d_group_offsets, int rows,
                             void* d_y, int y_dtype, size_t y_row_stride, void* stream) {
     if (!d_group_offsets) return -1;
-    return sb::product((sb::Mxfp4Weights*)weights, d_codes, d_scales, d_group_offsets, rows, d_y, y_dtype, y_row_stride,
+    return sb::product((sb::Mxfp4Handle*)weights, d_codes, d_scales, d_group_offsets, rows, d_y, y_dtype, y_row_stride,
                        (cudaStream_t)stream);
 }
 
 int salt_b200_mxfp4_status(void* weights, void* stream) {
     using namespace sb;
-    Mxfp4Weights* w = (Mxfp4Weights*)weights;
+    Mxfp4Handle* w = (Mxfp4Handle*)weights;
     if (!w || !on_device(w)) return -1;
     int status = 0;
     if (!cuda_ok(cudaMemcpyAsync(&status, w->status, sizeof status, cudaMemcpyDeviceToHost, (cudaStream_t)stream), "mxfp4 status") ||
