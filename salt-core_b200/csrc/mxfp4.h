@@ -1,26 +1,30 @@
 // MXFP4 weights on the device and the launches of their products.
 #pragma once
-#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace sb {
 
-// Layout made once at creation.  Codes: [experts][stored rows][cols / 2]; a gated pair is stored with its rows alternating (gate
-// row i at 2 i, up row i at 2 i + 1), so that the two values an activation needs lie side by side in every kernel.  Scales: per
-// 128 stored rows and 128 columns one tile of 512 bytes, the byte of row r and 32-column block k at (r % 32) * 16 + (r / 32) * 4 + k
-// (the order in which the tensor core reads them); tiles beyond the last row or column hold 127 = 2^0.
+// Layout made once at creation: per 128 stored rows and 256 columns one tile of 17 KB that a single bulk copy brings into shared
+// memory as the tensor core reads it, tiles of a row block next to one another.  (Rows of codes side by side, as they come, cost
+// 128 separate lines of 128 bytes per tile: 535 MB of experts then streamed at 3.7 TB/s.)
+//   16384 bytes of codes: row r at r * 128, its 16-byte piece c (one block of 32 columns) at place c ^ (r % 8);
+//   1024 bytes of scales: block c of row r at (c / 4) * 512 + (r % 32) * 16 + (r / 32) * 4 + c % 4.
+// A gated pair is stored with its rows alternating (gate row i at 2 i, up row i at 2 i + 1), so that the two values an activation
+// needs lie side by side in every kernel.  Rows and columns that fill a tile up have codes 0 and scales 127 = 2^0.
+constexpr int MX_TILE_ROWS = 128, MX_TILE_COLS = 256;
+constexpr int MX_CODE_BYTES = MX_TILE_ROWS * MX_TILE_COLS / 2;
+constexpr int MX_TILE_BYTES = MX_CODE_BYTES + MX_TILE_ROWS * MX_TILE_COLS / 32;
+
 struct Mxfp4Weights {
     int device;
     int rows, cols, experts;     // rows of the result; cols = K
     int stored_rows;             // rows, or 2 rows of a gated pair
-    int row_tiles, col_tiles;    // scale tiles of an expert; col_tiles is even
+    int row_tiles, chunks;       // tiles of an expert along rows and columns
     int activation;              // SALT_B200_ACT_*
-    uint8_t* codes;
-    uint8_t* scales;
+    uint8_t* tiles;              // [experts][row_tiles][chunks][MX_TILE_BYTES]
     int* status;
 };
-struct Mxfp4Handle : Mxfp4Weights { CUtensorMap map; };
 
 struct Mxfp4Call {
     const uint8_t* codes;        // [rows][cols / 2]
@@ -34,16 +38,22 @@ struct Mxfp4Call {
 
 // mxfp4_few_rows.cu: passes of up to eight rows, exact integer sums per block
 cudaError_t launch_mxfp4_few_rows(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
-
 // mxfp4_tensor.cu: block-scaled tensor-core products
-cudaError_t make_mxfp4_weight_map(CUtensorMap* out, const Mxfp4Weights& w);
-cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const CUtensorMap& weight_map, const Mxfp4Call& c, cudaStream_t stream);
+cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
 
 // y = act(gate) * up
 __device__ __forceinline__ float gate_act(int activation, float g) {
-    if (activation == 2) return g / (1.0f + expf(-g));                                                  // SiLU
-    const float t = tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g));                          // GELU, tanh form
-    return 0.5f * g * (1.0f + t);
+    // both are g / (1 + exp(-z)): z = g is SiLU, z = 2 sqrt(2 / pi) (g + 0.044715 g^3) the tanh form of GELU.  The fast exponential and
+    // quotient are off by a few units of 2^-24 |z| where exp(-z) matters, which against |g| stays below 2^-21
+    const float z = activation == 2 ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
+    return __fdividef(g, 1.0f + __expf(-z));
+}
+
+// Bulk copy of a tile (both addresses on 16 bytes, a multiple of 16 bytes) into this block's own shared memory.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(bar)
+                 : "memory");
 }
 
 }  // namespace sb

@@ -6,8 +6,8 @@
 // grid, a group's row tiles next to one another, so the blocks that work at the same time read the same activations.  Which
 // group a unit belongs to is found in a prefix table over the groups' passes, made by every block from the device offsets.
 // Warp roles:
-//   warp 9      producer: TMA copies of the weight codes (3-D map: byte column, row, expert), of the rows' codes (boxes of 32 rows)
-//               and of the weights' scale tiles, which lie in memory as the tensor core reads them
+//   warp 9      producer: one bulk copy of the weight tile, codes and scales, which lies in memory as the tensor core reads it, and
+//               TMA copies of the rows' codes (boxes of 32 rows, 128-byte swizzle)
 //   warps 0-3   scales of the rows: 16 bytes per row and pair of chunks, loaded a pair ahead, written to shared memory in the order
 //               of a scale tile
 //   warp 8      issuer: tcgen05.cp of the chunk's scale tiles to TMEM, then its four MMAs; both run in issue order
@@ -28,11 +28,10 @@ namespace {
 
 constexpr int MT_THREADS = 320;          // warps 0-3 scales, 4-7 epilogue, 8 issuer, 9 producer
 constexpr int MT_CHUNK = 128;            // packed bytes of a K chunk
-constexpr int MT_A_BYTES = 128 * MT_CHUNK;
 constexpr int MT_BOX = 32;               // rows of an activation copy
 constexpr int MT_MAX_N = 224;            // two accumulators of 224 columns and 64 columns of scales fill TMEM
 constexpr uint32_t MT_TMEM_COLS = 512, MT_SF_BASE = 448, MT_SF_STRIDE = 32, MT_SFB = 8;
-constexpr int MT_SFA_BYTES = 1024, MT_SFB_BYTES = 2048;
+constexpr int MT_SFB_BYTES = 2048;
 constexpr int MT_MAX_STAGES = 8;
 constexpr int MT_SMEM = 222 * 1024;
 
@@ -43,8 +42,6 @@ struct MxTensorArgs {
     int stages, stage_bytes;
     int chunks;
 };
-
-struct MxMaps { CUtensorMap w, x; };
 
 // kind::mxf4 instruction descriptor: A = B = E2M1, K-major, E8M0 scales, `half` = which two bytes of a scale word the MMA reads.
 __device__ __forceinline__ uint32_t mx_idesc(int N, uint32_t half) {
@@ -66,11 +63,15 @@ __device__ __forceinline__ void scale_copy(uint32_t taddr, uint32_t smem) {
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
-                 "r"(smem_u32(bar))
-                 : "memory");
+// One lane of a converged warp.  The instructions for copies and MMAs take their operands from the warp's uniform registers: inside
+// this election, with operands that are the same in all lanes, they are issued at once; under `lane == 0` the compiler has to
+// go through the lanes, and a chunk's four MMAs, six scale copies and commit took 1100 cycles.
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
+    return p != 0;
 }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 struct Unit { int expert, tile, row0, n, N; };   // n rows of the pass, N = n up to a multiple of 16
 
@@ -109,9 +110,17 @@ struct Groups {
         out->N = (out->n + 15) & ~15;
         return out->n > 0;
     }
+    __device__ __forceinline__ bool unit_uniform(int u, Unit* out) const {   // by a whole warp
+        const bool ok = uniform(unit(u, out));
+        out->expert = uniform(out->expert); out->tile = uniform(out->tile); out->row0 = uniform(out->row0);
+        out->n = uniform(out->n); out->N = uniform(out->N);
+        return ok;
+    }
 };
 
-__global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTensorArgs a, const __grid_constant__ MxMaps maps) {
+template <int FT, bool GATED>
+__global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTensorArgs a, const __grid_constant__ CUtensorMap xmap) {
+    using T = typename FloatType<FT>::T;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_free[MT_MAX_STAGES], bar_full[MT_MAX_STAGES], bar_sf[MT_MAX_STAGES];
     __shared__ __align__(8) uint64_t bar_done[2], bar_accfree[2], bar_drain;
@@ -120,7 +129,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
     __shared__ int s_first[1025];
     __shared__ int s_part[MT_THREADS / 32];
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
     uint8_t* stage_base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     volatile int* fail = &s_fail;
     if (tid == 0) {
@@ -178,86 +187,79 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     Groups groups;
     groups.first = a.c.offsets ? s_first : nullptr;
     groups.offsets = a.c.offsets; groups.experts = a.w.experts; groups.rows = a.c.rows; groups.cap = a.cap; groups.tiles = a.w.row_tiles;
     const int size = pass_rows(a.c.rows, a.cap);
     const int units = (a.c.offsets ? s_first[a.w.experts] : (a.c.rows + size - 1) / size) * a.w.row_tiles;
-    const int b_off = MT_A_BYTES, sfa_off = a.stage_bytes - MT_SFA_BYTES - MT_SFB_BYTES, sfb_off = a.stage_bytes - MT_SFB_BYTES;
+    const int sfb_off = a.stage_bytes - MT_SFB_BYTES;    // a stage: weight tile, rows' codes, rows' scales
 
+    const uint32_t stage0 = (uint32_t)uniform((int)smem_u32(stage_base));
     uint32_t produced = 0;
     if (warp == 9) {
         // ================= producer =================
-        if (lane == 0) {
-            bool ok = true;
-            uint32_t s = 0, ph = 1;                      // a fresh barrier's previous phase counts as complete
-            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-                Unit un;
-                if (!groups.unit(u, &un)) continue;
-                const int boxes = (un.N + MT_BOX - 1) / MT_BOX;
-                const uint32_t tx = MT_A_BYTES + MT_SFA_BYTES + boxes * (MT_BOX * MT_CHUNK);
-                const uint8_t* sfa = a.w.scales + ((size_t)un.expert * a.w.row_tiles + un.tile) * a.w.col_tiles * 512;
-                for (int kc = 0; kc < a.chunks; kc++, produced++) {
-                    if (!mbar_wait(&bar_free[s], ph, fail)) { ok = false; break; }
-                    const uint32_t dst = smem_u32(stage_base + s * a.stage_bytes);
+        uint32_t s = 0, ph = 1;                          // a fresh barrier's previous phase counts as complete
+        bool ok = true;
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            Unit un;
+            if (!groups.unit_uniform(u, &un)) continue;
+            const int boxes = (un.N + MT_BOX - 1) / MT_BOX;
+            const uint32_t tx = MX_TILE_BYTES + boxes * (MT_BOX * MT_CHUNK);
+            const uint8_t* tile = a.w.tiles + ((size_t)un.expert * a.w.row_tiles + un.tile) * a.chunks * MX_TILE_BYTES;
+            for (int kc = 0; kc < a.chunks; kc++, produced++) {
+                ok = mbar_wait(&bar_free[s], ph, fail);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (elected()) {
+                    const uint32_t dst = stage0 + s * a.stage_bytes;
                     mbar_expect_tx(&bar_full[s], tx);
-                    tma_load_3d(dst, &maps.w, kc * MT_CHUNK, un.tile * 128, un.expert, &bar_full[s]);
+                    bulk_load(dst, tile + (size_t)kc * MX_TILE_BYTES, MX_TILE_BYTES, smem_u32(&bar_full[s]));
                     for (int b = 0; b < boxes; b++)
-                        tma_load_2d(dst + b_off + b * (MT_BOX * MT_CHUNK), &maps.x, kc * MT_CHUNK, un.row0 + b * MT_BOX, &bar_full[s]);
-                    bulk_load(dst + sfa_off, sfa + (size_t)kc * 1024, MT_SFA_BYTES, &bar_full[s]);
-                    if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
+                        tma_load_2d(dst + MX_TILE_BYTES + b * (MT_BOX * MT_CHUNK), &xmap, kc * MT_CHUNK, un.row0 + b * MT_BOX, &bar_full[s]);
                 }
+                __syncwarp();
+                if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
             }
         }
-        __syncwarp();
     } else if (warp == 8) {
-        // ================= issuer (one thread) =================
-        // The barriers of the next stage are looked at before this stage's MMAs go out: a wait costs 150 to 250 cycles even
-        // when its phase is complete.
-        if (lane == 0) {
-            const uint32_t base = smem_u32(stage_base);
-            uint32_t s = 0, ph = 0, ready = 0, done = 0, par = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-                Unit un;
-                if (!groups.unit(u, &un)) continue;
-                const uint32_t buf = done & 1u;
-                if (done >= 2u) ok = mbar_wait(&bar_accfree[buf], ((done >> 1) - 1) & 1, fail);
-                const uint32_t id0 = mx_idesc(un.N, 0), id1 = mx_idesc(un.N, 1);
-                const uint32_t d = tmem + buf * MT_MAX_N;
-                const int halves = (un.N + 127) / 128;
-                for (int kc = 0; kc < a.chunks && ok; kc++) {
-                    if (!ready) ok = mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail);
-                    if (!ok) break;
-                    uint32_t ns = s + 1, nph = ph;
-                    if (ns == (uint32_t)a.stages) { ns = 0; nph ^= 1u; }
-                    const uint32_t r_full = mbar_test(&bar_full[ns], nph), r_sf = mbar_test(&bar_sf[ns], nph);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t st = base + s * a.stage_bytes;
-                    const uint32_t sf = tmem + MT_SF_BASE + par * MT_SF_STRIDE;
-                    par ^= 1u;
+        // ================= issuer =================
+        uint32_t s = 0, ph = 0, done = 0, par = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            Unit un;
+            if (!groups.unit_uniform(u, &un)) continue;
+            const uint32_t buf = done & 1u;
+            if (done >= 2u) ok = __all_sync(0xffffffffu, mbar_wait(&bar_accfree[buf], ((done >> 1) - 1) & 1, fail));
+            const uint32_t id0 = mx_idesc(un.N, 0), id1 = mx_idesc(un.N, 1);
+            const uint32_t d = tmem + buf * MT_MAX_N;
+            for (int kc = 0; kc < a.chunks && ok; kc++) {
+                ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t st = stage0 + s * a.stage_bytes;
+                const uint32_t sf = tmem + MT_SF_BASE + par * MT_SF_STRIDE;
+                par ^= 1u;
+                if (elected()) {
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        scale_copy(sf + 4 * k, st + sfa_off + k * 512);
+                        scale_copy(sf + 4 * k, st + MX_CODE_BYTES + k * 512);
                         scale_copy(sf + MT_SFB + 8 * k, st + sfb_off + k * 1024);
-                        if (halves > 1) scale_copy(sf + MT_SFB + 8 * k + 4, st + sfb_off + k * 1024 + 512);
+                        if (un.N > 128) scale_copy(sf + MT_SFB + 8 * k + 4, st + sfb_off + k * 1024 + 512);
                     }
-                    const uint32_t alo = DESC_B_LO | ((st & 0x3ffffu) >> 4), blo = alo + (b_off >> 4);
+                    const uint32_t alo = DESC_B_LO | ((st & 0x3ffffu) >> 4), blo = alo + (MX_TILE_BYTES >> 4);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         mx_mma(d, make_desc(alo + j * 2, DESC_B_HI), make_desc(blo + j * 2, DESC_B_HI), (j & 1) ? id1 : id0,
                                sf + 4 * (j >> 1), sf + MT_SFB + 8 * (j >> 1), (kc > 0 || j > 0) ? 1u : 0u);
                     umma_commit(&bar_free[s]);
                     if (kc == a.chunks - 1) umma_commit(&bar_done[buf]);
-                    ready = r_full & r_sf;
-                    s = ns;
-                    ph = nph;
                 }
-                done++;
+                __syncwarp();
+                if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
             }
+            done++;
         }
-        __syncwarp();
     } else if (warp < 4) {
         // ================= scales of the rows =================
         const int blocks = a.w.cols / 32;
@@ -329,21 +331,27 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
             for (int n0 = 0; n0 < un.N; n0 += 32) {
                 uint32_t acc[32];
                 tmem_ld32(trow + buf * MT_MAX_N + n0, acc);
-                const size_t row = (size_t)(un.row0 + n0);
-                if (a.w.activation) {
+                if (GATED) {
                     // lanes 2 i and 2 i + 1 hold gate and up of the same result: the even lane takes even rows, the odd lane odd ones
+                    const bool odd = lane & 1;
+                    T* y = (T*)a.c.y + (size_t)(un.row0 + n0 + odd) * a.c.y_stride + (m >> 1);
+                    const int left = live ? un.n - n0 - odd : 0;
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        const float mine = __uint_as_float((lane & 1) ? acc[k + 1] : acc[k]);
-                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float((lane & 1) ? acc[k] : acc[k + 1]), 1);
-                        const int n = n0 + k + (lane & 1);
-                        const float v = (lane & 1) ? gate_act(a.w.activation, other) * mine : gate_act(a.w.activation, mine) * other;
-                        if (live && n < un.n) store_float(a.c.y, a.c.y_type, (row + k + (lane & 1)) * a.c.y_stride + (m >> 1), v);
+                        const float mine = __uint_as_float(odd ? acc[k + 1] : acc[k]);
+                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? acc[k] : acc[k + 1]), 1);
+                        const float gate = odd ? other : mine, up = odd ? mine : other;
+                        if (k < left) *y = FloatType<FT>::down(gate_act(a.w.activation, gate) * up);
+                        y += 2 * a.c.y_stride;
                     }
                 } else {
+                    T* y = (T*)a.c.y + (size_t)(un.row0 + n0) * a.c.y_stride + m;
+                    const int left = live ? un.n - n0 : 0;
 #pragma unroll
-                    for (int k = 0; k < 32; k++)
-                        if (live && n0 + k < un.n) store_float(a.c.y, a.c.y_type, (row + k) * a.c.y_stride + m, __uint_as_float(acc[k]));
+                    for (int k = 0; k < 32; k++) {
+                        if (k < left) *y = FloatType<FT>::down(__uint_as_float(acc[k]));
+                        y += a.c.y_stride;
+                    }
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -376,44 +384,35 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
 
 }  // namespace
 
-cudaError_t make_mxfp4_weight_map(CUtensorMap* out, const Mxfp4Weights& w) {
-    TensorMapEncodeFn encode = nullptr;
-    const cudaError_t e = tensor_map_encoder(&encode);
-    if (e != cudaSuccess) return e;
-    const cuuint64_t row = (cuuint64_t)w.cols / 2;
-    cuuint64_t dims[3] = {row, (cuuint64_t)w.stored_rows, (cuuint64_t)w.experts};
-    cuuint64_t strides[2] = {row, row * w.stored_rows};
-    cuuint32_t box[3] = {(cuuint32_t)MT_CHUNK, 128u, 1u}, estr[3] = {1, 1, 1};
-    return encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, w.codes, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
-               ? cudaSuccess
-               : cudaErrorInvalidValue;
-}
-
-cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const CUtensorMap& weight_map, const Mxfp4Call& c, cudaStream_t stream) {
+cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream) {
     TensorMapEncodeFn encode = nullptr;
     cudaError_t e = tensor_map_encoder(&encode);
     if (e != cudaSuccess) return e;
-    MxMaps maps;
-    maps.w = weight_map;
+    CUtensorMap xmap;
     cuuint64_t dims[2] = {(cuuint64_t)w.cols / 2, (cuuint64_t)c.rows}, strides[1] = {(cuuint64_t)w.cols / 2};
     cuuint32_t box[2] = {(cuuint32_t)MT_CHUNK, (cuuint32_t)MT_BOX}, estr[2] = {1, 1};
-    if (encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(c.codes), dims, strides, box, estr,
+    if (encode(&xmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(c.codes), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
     MxTensorArgs a;
     a.w = w;
     a.c = c;
-    a.cap = MT_MAX_N;
-    a.chunks = (w.cols + 255) / 256;
-    a.stage_bytes = MT_A_BYTES + a.cap * MT_CHUNK + MT_SFA_BYTES + MT_SFB_BYTES;
+    a.cap = MT_MAX_N; 
+    a.chunks = w.chunks;
+    a.stage_bytes = MX_TILE_BYTES + a.cap * MT_CHUNK + MT_SFB_BYTES;
     a.stages = std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes);
     const size_t smem = (size_t)a.stages * a.stage_bytes + 1024;
-    if ((e = ensure_dynamic_smem((const void*)mxfp4_tensor_kernel, smem)) != cudaSuccess) return e;
     const long long passes = c.offsets ? (long long)c.rows / a.cap + std::min(c.rows, w.experts) + 1 : (c.rows + a.cap - 1) / a.cap + 1;
     const int grid = (int)std::min<long long>(device_sms(), passes * w.row_tiles);
-    return launch_pdl(mxfp4_tensor_kernel, dim3(grid), dim3(MT_THREADS), smem, stream, a, maps);
+    const auto kernel = w.activation ? (c.y_type == FT_F32    ? mxfp4_tensor_kernel<FT_F32, true>
+                                        : c.y_type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, true>
+                                                              : mxfp4_tensor_kernel<FT_F16, true>)
+                                     : (c.y_type == FT_F32    ? mxfp4_tensor_kernel<FT_F32, false>
+                                        : c.y_type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, false>
+                                                              : mxfp4_tensor_kernel<FT_F16, false>);
+    if ((e = ensure_dynamic_smem((const void*)kernel, smem)) != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3(grid), dim3(MT_THREADS), smem, stream, a, xmap);
 }
 
 }  // namespace sb
