@@ -335,22 +335,32 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
                     // lanes 2 i and 2 i + 1 hold gate and up of the same result: the even lane takes even rows, the odd lane odd ones
                     const bool odd = lane & 1;
                     T* y = (T*)a.c.y + (size_t)(un.row0 + n0 + odd) * a.c.y_stride + (m >> 1);
-                    const int left = live ? un.n - n0 - odd : 0;
+                    const int left = live ? un.n - n0 - odd : 0;     // rows k = 0, 2, ... below it exist
+                    float v[16];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float mine = __uint_as_float(odd ? acc[k + 1] : acc[k]);
-                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? acc[k] : acc[k + 1]), 1);
-                        const float gate = odd ? other : mine, up = odd ? mine : other;
-                        if (k < left) *y = FloatType<FT>::down(gate_act(a.w.activation, gate) * up);
-                        y += 2 * a.c.y_stride;
+                    for (int k = 0; k < 16; k++) {
+                        const float mine = __uint_as_float(odd ? acc[2 * k + 1] : acc[2 * k]);
+                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? acc[2 * k] : acc[2 * k + 1]), 1);
+                        v[k] = gate_act(a.w.activation, odd ? other : mine) * (odd ? mine : other);
+                    }
+                    if (left >= 31) {                    // all 32 rows: no branch between the activations
+#pragma unroll
+                        for (int k = 0; k < 16; k++) y[(size_t)(2 * k) * a.c.y_stride] = FloatType<FT>::down(v[k]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; k++)
+                            if (2 * k < left) y[(size_t)(2 * k) * a.c.y_stride] = FloatType<FT>::down(v[k]);
                     }
                 } else {
                     T* y = (T*)a.c.y + (size_t)(un.row0 + n0) * a.c.y_stride + m;
                     const int left = live ? un.n - n0 : 0;
+                    if (left >= 32) {
 #pragma unroll
-                    for (int k = 0; k < 32; k++) {
-                        if (k < left) *y = FloatType<FT>::down(__uint_as_float(acc[k]));
-                        y += a.c.y_stride;
+                        for (int k = 0; k < 32; k++) y[(size_t)k * a.c.y_stride] = FloatType<FT>::down(__uint_as_float(acc[k]));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; k++)
+                            if (k < left) y[(size_t)k * a.c.y_stride] = FloatType<FT>::down(__uint_as_float(acc[k]));
                     }
                 }
             }
