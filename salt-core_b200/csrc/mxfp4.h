@@ -36,10 +36,8 @@ struct Mxfp4Call {
     size_t y_stride;
 };
 
-// mxfp4_few_rows.cu: passes of up to eight rows, exact integer sums per block
-cudaError_t launch_mxfp4_few_rows(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
-// mxfp4_tensor.cu: block-scaled tensor-core products
-cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
+// mxfp4_tensor.cu: any number of rows
+cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
 
 // y = act(gate) * up
 __device__ __forceinline__ float gate_act(int activation, float g) {

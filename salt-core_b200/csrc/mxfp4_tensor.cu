@@ -5,6 +5,7 @@
 // 128-byte row of packed codes = four MMAs of K = 64.  Persistent blocks, one per SM; unit u of the launch goes to block u mod
 // grid, a group's row tiles next to one another, so the blocks that work at the same time read the same activations.  Which
 // group a unit belongs to is found in a prefix table over the groups' passes, made by every block from the device offsets.
+// Where the units are few, a cluster of 2 to 8 blocks shares each, K split; the partial sums meet in distributed shared memory.
 // Warp roles:
 //   warp 9      producer: one bulk copy of the weight tile, codes and scales, which lies in memory as the tensor core reads it, and
 //               TMA copies of the rows' codes (boxes of 32 rows, 128-byte swizzle)
@@ -14,6 +15,8 @@
 //   warps 4-7   epilogue: lane = weight row, column = row of the result; a gated pair's two rows are neighbouring lanes
 // Every mbarrier wait is bounded; on expiry the block raises its failure flag, sets SB_ERR_TIMEOUT, waits (bounded) for copies
 // and MMAs in flight, frees its TMEM and returns.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "../../include/salt_gpu_b200.h"
@@ -23,6 +26,8 @@
 #include "pdl.cuh"
 #include "umma.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace sb {
 namespace {
 
@@ -30,17 +35,20 @@ constexpr int MT_THREADS = 320;          // warps 0-3 scales, 4-7 epilogue, 8 is
 constexpr int MT_CHUNK = 128;            // packed bytes of a K chunk
 constexpr int MT_BOX = 32;               // rows of an activation copy
 constexpr int MT_MAX_N = 224;            // two accumulators of 224 columns and 64 columns of scales fill TMEM
-constexpr uint32_t MT_TMEM_COLS = 512, MT_SF_BASE = 448, MT_SF_STRIDE = 32, MT_SFB = 8;
+constexpr int MT_SMALL_N = 64;           // two of 64 columns and the scales half of it: two blocks per SM
+constexpr uint32_t MT_SF_STRIDE = 32, MT_SFB = 8;
 constexpr int MT_SFB_BYTES = 2048;
 constexpr int MT_MAX_STAGES = 8;
-constexpr int MT_SMEM = 222 * 1024;
+constexpr int MT_MAX_SPLIT = 8;
+constexpr int MT_SMEM = 220 * 1024, MT_SMALL_SMEM = 103 * 1024;
 
 struct MxTensorArgs {
     Mxfp4Weights w;
     Mxfp4Call c;
     int cap;                             // most rows of a pass, a multiple of 16
     int stages, stage_bytes;
-    int chunks;
+    uint32_t tmem_cols, acc_cols;        // columns of TMEM, and of one of the two accumulators at its start
+    int split, share;                    // blocks of a cluster that share a unit, and most of its chunks that one takes
 };
 
 // kind::mxf4 instruction descriptor: A = B = E2M1, K-major, E8M0 scales, `half` = which two bytes of a scale word the MMA reads.
@@ -82,8 +90,7 @@ __device__ __forceinline__ int pass_rows(int n, int cap) {
 }
 
 struct Groups {
-    const int* first;                    // [experts + 1] passes before each group (shared memory), null for one dense matrix
-    const int32_t* offsets;
+    const int *first, *begin;            // [experts + 1] passes before a group and its first row (shared memory); null for one dense matrix
     int experts, rows, cap, tiles;
 
     __device__ __forceinline__ bool unit(int u, Unit* out) const {
@@ -100,8 +107,8 @@ struct Groups {
             }
             e = lo;
             p = pass - first[e];
-            b = max(offsets[e], 0);
-            t = min(offsets[e + 1], rows);
+            b = begin[e];
+            t = min(begin[e + 1], rows);
         }
         const int size = pass_rows(t - b, cap);
         out->expert = e;
@@ -119,14 +126,14 @@ struct Groups {
 };
 
 template <int FT, bool GATED>
-__global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTensorArgs a, const __grid_constant__ CUtensorMap xmap) {
+__global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTensorArgs a, const __grid_constant__ CUtensorMap xmap) {
     using T = typename FloatType<FT>::T;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bar_free[MT_MAX_STAGES], bar_full[MT_MAX_STAGES], bar_sf[MT_MAX_STAGES];
     __shared__ __align__(8) uint64_t bar_done[2], bar_accfree[2], bar_drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
-    __shared__ int s_first[1025];
+    __shared__ int s_first[1025], s_begin[1025];         // passes before a group, where it begins
     __shared__ int s_part[MT_THREADS / 32];
 
     const int tid = threadIdx.x, warp = uniform(tid >> 5), lane = tid & 31;
@@ -147,20 +154,23 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(MT_TMEM_COLS)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(a.tmem_cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    pdl_wait();
-    pdl_launch_dependents();
+    // A dense product's weights do not wait for the launch before: the producer asks for them first.
     if (a.c.offsets) {
+        pdl_wait();
+        pdl_launch_dependents();
         // passes before every group: a thread sums a run of groups, then the threads' sums are scanned
         const int run = (a.w.experts + MT_THREADS - 1) / MT_THREADS;
         int sum = 0;
         for (int j = 0; j < run; j++) {
             const int e = tid * run + j;
             if (e >= a.w.experts) break;
-            const int n = min(a.c.offsets[e + 1], a.c.rows) - max(a.c.offsets[e], 0);
+            const int b = max(a.c.offsets[e], 0), t = a.c.offsets[e + 1], n = min(t, a.c.rows) - b;
+            s_begin[e] = b;
+            if (e == a.w.experts - 1) s_begin[e + 1] = t;
             s_first[e] = sum;
             if (n > 0) {
                 const int size = pass_rows(n, a.cap);
@@ -190,9 +200,11 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
     const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     Groups groups;
     groups.first = a.c.offsets ? s_first : nullptr;
-    groups.offsets = a.c.offsets; groups.experts = a.w.experts; groups.rows = a.c.rows; groups.cap = a.cap; groups.tiles = a.w.row_tiles;
+    groups.begin = s_begin; groups.experts = a.w.experts; groups.rows = a.c.rows; groups.cap = a.cap; groups.tiles = a.w.row_tiles;
     const int size = pass_rows(a.c.rows, a.cap);
     const int units = (a.c.offsets ? s_first[a.w.experts] : (a.c.rows + size - 1) / size) * a.w.row_tiles;
+    const int rank = a.split > 1 ? (int)(blockIdx.x % a.split) : 0, first_unit = (int)blockIdx.x / a.split, unit_step = (int)gridDim.x / a.split;
+    const int kc0 = rank * a.share, kc1 = min(a.w.chunks, kc0 + a.share);
     const int sfb_off = a.stage_bytes - MT_SFB_BYTES;    // a stage: weight tile, rows' codes, rows' scales
 
     const uint32_t stage0 = (uint32_t)uniform((int)smem_u32(stage_base));
@@ -200,21 +212,36 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
     if (warp == 9) {
         // ================= producer =================
         uint32_t s = 0, ph = 1;                          // a fresh barrier's previous phase counts as complete
-        bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        bool ok = true, waited = a.c.offsets != nullptr;
+        for (int u = first_unit; u < units && ok; u += unit_step) {
             Unit un;
             if (!groups.unit_uniform(u, &un)) continue;
             const int boxes = (un.N + MT_BOX - 1) / MT_BOX;
             const uint32_t tx = MX_TILE_BYTES + boxes * (MT_BOX * MT_CHUNK);
-            const uint8_t* tile = a.w.tiles + ((size_t)un.expert * a.w.row_tiles + un.tile) * a.chunks * MX_TILE_BYTES;
-            for (int kc = 0; kc < a.chunks; kc++, produced++) {
+            const uint8_t* tile = a.w.tiles + ((size_t)un.expert * a.w.row_tiles + un.tile) * a.w.chunks * MX_TILE_BYTES;
+            int early = kc0;                             // weights of the chunks below have been asked for
+            if (!waited) {
+                early = min(kc1, kc0 + a.stages);
+                if (elected())
+                    for (int k = 0; k < early - kc0; k++) {
+                        mbar_expect_tx(&bar_full[k], tx);
+                        bulk_load(stage0 + k * a.stage_bytes, tile + (size_t)(kc0 + k) * MX_TILE_BYTES, MX_TILE_BYTES, smem_u32(&bar_full[k]));
+                    }
+                __syncwarp();
+                pdl_wait();
+                pdl_launch_dependents();
+                waited = true;
+            }
+            for (int kc = kc0; kc < kc1; kc++, produced++) {
                 ok = mbar_wait(&bar_free[s], ph, fail);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 if (elected()) {
                     const uint32_t dst = stage0 + s * a.stage_bytes;
-                    mbar_expect_tx(&bar_full[s], tx);
-                    bulk_load(dst, tile + (size_t)kc * MX_TILE_BYTES, MX_TILE_BYTES, smem_u32(&bar_full[s]));
+                    if (kc >= early) {
+                        mbar_expect_tx(&bar_full[s], tx);
+                        bulk_load(dst, tile + (size_t)kc * MX_TILE_BYTES, MX_TILE_BYTES, smem_u32(&bar_full[s]));
+                    }
                     for (int b = 0; b < boxes; b++)
                         tma_load_2d(dst + MX_TILE_BYTES + b * (MT_BOX * MT_CHUNK), &xmap, kc * MT_CHUNK, un.row0 + b * MT_BOX, &bar_full[s]);
                 }
@@ -226,19 +253,23 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
         // ================= issuer =================
         uint32_t s = 0, ph = 0, done = 0, par = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        if (!a.c.offsets) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
+        for (int u = first_unit; u < units && ok; u += unit_step) {
             Unit un;
             if (!groups.unit_uniform(u, &un)) continue;
             const uint32_t buf = done & 1u;
             if (done >= 2u) ok = __all_sync(0xffffffffu, mbar_wait(&bar_accfree[buf], ((done >> 1) - 1) & 1, fail));
             const uint32_t id0 = mx_idesc(un.N, 0), id1 = mx_idesc(un.N, 1);
-            const uint32_t d = tmem + buf * MT_MAX_N;
-            for (int kc = 0; kc < a.chunks && ok; kc++) {
+            const uint32_t d = tmem + buf * a.acc_cols;
+            for (int kc = kc0; kc < kc1 && ok; kc++) {
                 ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t st = stage0 + s * a.stage_bytes;
-                const uint32_t sf = tmem + MT_SF_BASE + par * MT_SF_STRIDE;
+                const uint32_t sf = tmem + 2 * a.acc_cols + par * MT_SF_STRIDE;
                 par ^= 1u;
                 if (elected()) {
 #pragma unroll
@@ -251,9 +282,9 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         mx_mma(d, make_desc(alo + j * 2, DESC_B_HI), make_desc(blo + j * 2, DESC_B_HI), (j & 1) ? id1 : id0,
-                               sf + 4 * (j >> 1), sf + MT_SFB + 8 * (j >> 1), (kc > 0 || j > 0) ? 1u : 0u);
+                               sf + 4 * (j >> 1), sf + MT_SFB + 8 * (j >> 1), (kc > kc0 || j > 0) ? 1u : 0u);
                     umma_commit(&bar_free[s]);
-                    if (kc == a.chunks - 1) umma_commit(&bar_done[buf]);
+                    if (kc == kc1 - 1) umma_commit(&bar_done[buf]);
                 }
                 __syncwarp();
                 if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
@@ -262,11 +293,15 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
         }
     } else if (warp < 4) {
         // ================= scales of the rows =================
+        if (!a.c.offsets) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
         const int blocks = a.w.cols / 32;
         const size_t pitch = ((size_t)blocks + 15) / 16 * 16;
         uint32_t s = 0, ph = 1;
         bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        for (int u = first_unit; u < units && ok; u += unit_step) {
             Unit un;
             if (!groups.unit(u, &un)) continue;
             const int r0 = tid, r1 = tid + 128;
@@ -274,13 +309,17 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
             const uint4 one = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
             const uint4* p0 = (const uint4*)(a.c.scales + (size_t)(un.row0 + (have0 ? r0 : 0)) * pitch);
             const uint4* p1 = (const uint4*)(a.c.scales + (size_t)(un.row0 + (have1 ? r1 : 0)) * pitch);
-            uint4 n0 = have0 ? p0[0] : one, n1 = have1 ? p1[0] : one, c0 = n0, c1 = n1;
+            uint4 n0 = one, n1 = one, c0, c1;
+            if (have0 && kc0 < kc1) n0 = p0[kc0 >> 1];
+            if (have1 && kc0 < kc1) n1 = p1[kc0 >> 1];
+            c0 = n0;
+            c1 = n1;
             const uint32_t at0 = (r0 & 31) * 16 + (r0 >> 5) * 4;     // r1: the same in the second 512 bytes
-            for (int kc = 0; kc < a.chunks && ok; kc++) {
-                if (!(kc & 1)) {
+            for (int kc = kc0; kc < kc1 && ok; kc++) {
+                if (!(kc & 1) || kc == kc0) {
                     c0 = n0;
                     c1 = n1;
-                    if (kc + 2 < a.chunks) {
+                    if ((kc | 1) + 1 < kc1) {
                         if (have0) n0 = p0[(kc >> 1) + 1];
                         if (have1) n1 = p1[(kc >> 1) + 1];
                     }
@@ -318,9 +357,14 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
         const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
         uint32_t done = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        if (!a.c.offsets) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
+        for (int u = first_unit; u < units && ok; u += unit_step) {
             Unit un;
             if (!groups.unit(u, &un)) continue;
+            if (kc0 >= kc1) continue;                    // this block of the cluster has no chunks
             const int m = un.tile * 128 + q * 32 + lane;
             const bool live = m < a.w.stored_rows;
             const uint32_t buf = done & 1u;
@@ -330,8 +374,14 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int n0 = 0; n0 < un.N; n0 += 32) {
                 uint32_t acc[32];
-                tmem_ld32(trow + buf * MT_MAX_N + n0, acc);
-                if (GATED) {
+                tmem_ld32(trow + buf * a.acc_cols + n0, acc);
+                if (a.split > 1) {
+                    // the ring is idle after a cluster's only unit: partial sums [row of the result][128] go there
+                    float* part = (float*)stage_base + n0 * MX_TILE_ROWS + q * 32 + lane;
+#pragma unroll
+                    for (int k = 0; k < 32; k++)
+                        if (n0 + k < un.N) part[k * MX_TILE_ROWS] = __uint_as_float(acc[k]);
+                } else if (GATED) {
                     // lanes 2 i and 2 i + 1 hold gate and up of the same result: the even lane takes even rows, the odd lane odd ones
                     const bool odd = lane & 1;
                     T* y = (T*)a.c.y + (size_t)(un.row0 + n0 + odd) * a.c.y_stride + (m >> 1);
@@ -371,6 +421,33 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
         }
     }
 
+    if (a.split > 1) {
+        // The cluster's partial sums, added in rank order; the rows of the result are dealt out to its blocks.
+        const cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        Unit un;
+        if (first_unit < units && groups.unit(first_unit, &un)) {
+            const int live = (a.w.chunks + a.share - 1) / a.share;
+            for (int i = rank * MT_THREADS + tid; i < un.n * (MX_TILE_ROWS / 2); i += a.split * MT_THREADS) {
+                const int n = i / (MX_TILE_ROWS / 2), p = i - n * (MX_TILE_ROWS / 2), m = un.tile * MX_TILE_ROWS + 2 * p;
+                if (m >= a.w.stored_rows) continue;
+                float2 v = make_float2(0.f, 0.f);
+                for (int k = 0; k < live; k++) {
+                    const float2 o = *(const float2*)(cluster.map_shared_rank((float*)stage_base, k) + n * MX_TILE_ROWS + 2 * p);
+                    v.x += o.x;
+                    v.y += o.y;
+                }
+                T* y = (T*)a.c.y + (size_t)(un.row0 + n) * a.c.y_stride;
+                if (GATED) {
+                    y[m >> 1] = FloatType<FT>::down(gate_act(a.w.activation, v.x) * v.y);
+                } else {
+                    y[m] = FloatType<FT>::down(v.x);
+                    if (m + 1 < a.w.stored_rows) y[m + 1] = FloatType<FT>::down(v.y);
+                }
+            }
+        }
+        cluster.sync();                                  // a block's sums are read by the others until here
+    }
     __syncthreads();
     if (*fail) {
         if (tid == 0) atomicOr(a.w.status, SB_ERR_TIMEOUT);
@@ -389,12 +466,12 @@ __global__ void __launch_bounds__(MT_THREADS, 1) mxfp4_tensor_kernel(const MxTen
         __syncthreads();
     }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(MT_TMEM_COLS) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
 }
 
 }  // namespace
 
-cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream) {
+cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream) {
     TensorMapEncodeFn encode = nullptr;
     cudaError_t e = tensor_map_encoder(&encode);
     if (e != cudaSuccess) return e;
@@ -408,13 +485,24 @@ cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const Mxfp4Call& c, cudaS
     MxTensorArgs a;
     a.w = w;
     a.c = c;
-    a.cap = MT_MAX_N; 
-    a.chunks = w.chunks;
+    // Rows of a pass.  A dense product takes what it has; groups are seldom three times the average, and a pass more reads its
+    // weights again, from L2.  Fewer rows leave room for more stages.
+    const int expect = c.offsets ? std::min(c.rows, 3 * ((c.rows + w.experts - 1) / w.experts)) : c.rows;
+    a.cap = std::min(MT_MAX_N, (expect + MT_BOX - 1) / MT_BOX * MT_BOX);
     a.stage_bytes = MX_TILE_BYTES + a.cap * MT_CHUNK + MT_SFB_BYTES;
-    a.stages = std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes);
+    const bool small = a.cap <= MT_SMALL_N;
+    a.acc_cols = small ? MT_SMALL_N : MT_MAX_N;
+    a.tmem_cols = small ? 256 : 512;
+    a.stages = std::min(MT_MAX_STAGES, ((small ? MT_SMALL_SMEM : MT_SMEM) - 1024) / a.stage_bytes);
+    // Few units: a cluster shares one, a block at least two chunks
+    const long long passes = c.offsets ? std::min<long long>(c.rows, c.rows / a.cap + w.experts) : (c.rows + a.cap - 1) / a.cap;
+    const long long units = passes * w.row_tiles;
+    const int blocks = device_sms() * (small ? 2 : 1);
+    a.split = 1;
+    while (a.split < MT_MAX_SPLIT && units * a.split * 2 <= blocks && a.split * 4 <= w.chunks) a.split *= 2;
+    a.share = (w.chunks + a.split - 1) / a.split;
     const size_t smem = (size_t)a.stages * a.stage_bytes + 1024;
-    const long long passes = c.offsets ? (long long)c.rows / a.cap + std::min(c.rows, w.experts) + 1 : (c.rows + a.cap - 1) / a.cap + 1;
-    const int grid = (int)std::min<long long>(device_sms(), passes * w.row_tiles);
+    const int grid = a.split > 1 ? (int)units * a.split : (int)std::min<long long>(blocks, units);
     const auto kernel = w.activation ? (c.y_type == FT_F32    ? mxfp4_tensor_kernel<FT_F32, true>
                                         : c.y_type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, true>
                                                               : mxfp4_tensor_kernel<FT_F16, true>)
@@ -422,7 +510,21 @@ cudaError_t launch_mxfp4_tensor(const Mxfp4Weights& w, const Mxfp4Call& c, cudaS
                                         : c.y_type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, false>
                                                               : mxfp4_tensor_kernel<FT_F16, false>);
     if ((e = ensure_dynamic_smem((const void*)kernel, smem)) != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3(grid), dim3(MT_THREADS), smem, stream, a, xmap);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(MT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    if ((e = cudaLaunchKernelEx(&cfg, kernel, a, xmap)) == cudaSuccess) count_launches(1);
+    return e;
 }
 
 }  // namespace sb

@@ -93,8 +93,7 @@ int product(Mxfp4Weights* w, const uint8_t* codes, const uint8_t* scales, const 
     if (!codes || !scales || !y || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)y % float_type_size(y_type)) return -1;
     Mxfp4Call c;
     c.codes = codes; c.scales = scales; c.offsets = offsets; c.rows = rows; c.y = y; c.y_type = y_type; c.y_stride = y_stride;
-    const bool few = rows <= (offsets ? 2 * w->experts : 8);
-    return cuda_ok(few ? launch_mxfp4_few_rows(*w, c, stream) : launch_mxfp4_tensor(*w, c, stream), "mxfp4 product") ? 0 : -1;
+    return cuda_ok(launch_mxfp4_product(*w, c, stream), "mxfp4 product") ? 0 : -1;
 }
 
 }  // namespace
