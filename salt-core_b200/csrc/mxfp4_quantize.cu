@@ -20,7 +20,7 @@ bool cuda_ok(cudaError_t e, const char* what);
 
 namespace {
 
-constexpr int MQ_THREADS = 128;
+constexpr int MQ_MAX_THREADS = 256;
 
 struct QuantArgs {
     const void* x;
@@ -33,61 +33,89 @@ struct QuantArgs {
     void* values;
 };
 
-template <int FT, bool VALUES> __global__ void __launch_bounds__(MQ_THREADS) mxfp4_quantize_kernel(const QuantArgs a) {
+// A block works on one row, a thread on U pieces of eight columns, whose loads are all in flight before the first is used.
+template <int FT, bool VALUES, int U> __global__ void __launch_bounds__(MQ_MAX_THREADS) mxfp4_quantize_kernel(const QuantArgs a) {
     using T = typename FloatType<FT>::T;
     pdl_wait();
     pdl_launch_dependents();
     const int row = blockIdx.x;
-    long long src = a.index ? (long long)a.index[row] : row;
-    if (src < 0) return;                                 // an index below zero leaves its row as it was
-    src /= a.div;
-    if (src >= a.src_rows) return;
-    const int unit = blockIdx.y * MQ_THREADS + threadIdx.x;          // eight columns
-    const bool live = unit * 8 < a.cols;                 // the four lanes of a block agree
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (live) load8<FT>((const T*)a.x + (size_t)src * a.stride + unit * 8, v);
-    uint32_t top = 0;                                    // magnitudes order like their bits, NaN above infinity
-#pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (!live) return;
-    const uint32_t ex = top >> 23;                       // biased exponent; 0: subnormal or zero
-    const bool bad = ex == 255u;
-    const uint32_t s = bad ? 255u : (ex > 2u ? ex - 2u : 0u);
-    const float up = __uint_as_float((254u - min(s, 253u)) << 23);   // 2^(127 - s); s is at most 252 unless bad
-    uint32_t packed = 0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float lo = bad ? 0.f : __fmul_rn(v[2 * i], up), hi = bad ? 0.f : __fmul_rn(v[2 * i + 1], up);
-        uint32_t b;
-        asm("{ .reg .b8 q;\n\t"
-            "cvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\t"
-            "cvt.u32.u8 %0, q; }\n"
-            : "=r"(b)
-            : "f"(lo), "f"(hi));
-        packed |= b << (8 * i);
+    int src = row;
+    if (a.index) {
+        src = __ldg(a.index + row);
+        if (src < 0) return;                             // an index below zero leaves its row as it was
+        src = (int)((unsigned)src / (unsigned)a.div);
     }
-    *(uint32_t*)(a.codes + (size_t)row * (a.cols / 2) + unit * 4) = packed;
-    if ((unit & 3) == 0) a.scales[(size_t)row * a.pitch + (unit >> 2)] = (uint8_t)s;
-    if (VALUES) {
-        // magnitude of a code: bits m e1 e0 -> by arithmetic on the exponent; 2^(s - 127) has s = 0 as a subnormal
-        const float unit_value = __uint_as_float(s == 0u || s == 255u ? (s << 23) | 0x400000u : s << 23);
-        float o[8];
+    if (src >= a.src_rows) return;
+    const T* x = (const T*)a.x + (size_t)src * a.stride;
+    const int first = blockIdx.y * U * blockDim.x + threadIdx.x, units = a.cols / 8;
+    float v[U][8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t c = (packed >> (4 * i)) & 15u, e = (c >> 1) & 3u, m = c & 1u;
-            const float mag = e ? __uint_as_float(((126u + e) << 23) | (m << 22)) : 0.5f * (float)m;
-            o[i] = __fmul_rn(c & 8u ? -mag : mag, unit_value);
+    for (int u = 0; u < U; u++) {
+        const int unit = first + u * blockDim.x;         // the four lanes of a block of 32 columns agree on it
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[u][i] = 0.f;
+        if (unit < units) load8<FT>(x + unit * 8, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int unit = first + u * blockDim.x;
+        uint32_t top = 0;                                // magnitudes order like their bits, NaN above infinity
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t ex = top >> 23;                   // biased exponent; 0: subnormal or zero
+        const bool bad = ex == 255u;
+        const uint32_t s = bad ? 255u : (ex > 2u ? ex - 2u : 0u);
+        const float up = __uint_as_float((254u - min(s, 253u)) << 23);   // 2^(127 - s); s is at most 252 unless bad
+        uint32_t packed = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t b;
+            asm("{ .reg .b8 q;\n\t"
+                "cvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\t"
+                "cvt.u32.u8 %0, q; }\n"
+                : "=r"(b)
+                : "f"(__fmul_rn(v[u][2 * i], up)), "f"(__fmul_rn(v[u][2 * i + 1], up)));
+            packed |= b << (8 * i);
         }
-        store8<FT>((T*)a.values + (size_t)row * a.cols + unit * 8, o);
+        if (bad) packed = 0;
+        if (unit >= units) continue;
+        *(uint32_t*)(a.codes + (size_t)row * (a.cols / 2) + unit * 4) = packed;
+        if ((unit & 3) == 0) a.scales[(size_t)row * a.pitch + (unit >> 2)] = (uint8_t)s;
+        if (VALUES) {
+            const float unit_value = __uint_as_float(s == 0u || s == 255u ? (s << 23) | 0x400000u : s << 23);     // 2^(s - 127); NaN
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint32_t h;                              // two codes as halves, exactly
+                asm("{ .reg .b8 q;\n\t"
+                    "cvt.u8.u32 q, %1;\n\t"
+                    "cvt.rn.f16x2.e2m1x2 %0, q; }\n"
+                    : "=r"(h)
+                    : "r"(packed >> (8 * i)));
+                const float2 f = __half22float2(*(const __half2*)&h);
+                o[2 * i] = __fmul_rn(f.x, unit_value);
+                o[2 * i + 1] = __fmul_rn(f.y, unit_value);
+            }
+            store8<FT>((T*)a.values + (size_t)row * a.cols + unit * 8, o);
+        }
     }
 }
 
+template <int FT, bool VALUES> cudaError_t launch_quantize(const QuantArgs& a, cudaStream_t stream) {
+    const int units = a.cols / 8;
+    // four pieces per thread where the rows fill the SMs, one where a call is nothing but latency
+    const int per = a.rows >= 4 * device_sms() ? 4 : 1;
+    const int blocks = (units + MQ_MAX_THREADS * per - 1) / (MQ_MAX_THREADS * per);
+    const int threads = (((units + blocks - 1) / blocks + per - 1) / per + 31) / 32 * 32;
+    const dim3 grid(a.rows, blocks);
+    return per == 4 ? launch_pdl(mxfp4_quantize_kernel<FT, VALUES, 4>, grid, dim3(threads), 0, stream, a)
+                    : launch_pdl(mxfp4_quantize_kernel<FT, VALUES, 1>, grid, dim3(threads), 0, stream, a);
+}
+
 template <int FT> cudaError_t launch_quantize(const QuantArgs& a, cudaStream_t stream) {
-    const dim3 grid(a.rows, (a.cols / 8 + MQ_THREADS - 1) / MQ_THREADS);
-    return a.values ? launch_pdl(mxfp4_quantize_kernel<FT, true>, grid, dim3(MQ_THREADS), 0, stream, a)
-                    : launch_pdl(mxfp4_quantize_kernel<FT, false>, grid, dim3(MQ_THREADS), 0, stream, a);
+    return a.values ? launch_quantize<FT, true>(a, stream) : launch_quantize<FT, false>(a, stream);
 }
 
 }  // namespace

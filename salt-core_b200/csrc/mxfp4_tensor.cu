@@ -35,7 +35,7 @@ constexpr int MT_THREADS = 320;          // warps 0-3 scales, 4-7 epilogue, 8 is
 constexpr int MT_CHUNK = 128;            // packed bytes of a K chunk
 constexpr int MT_BOX = 32;               // rows of an activation copy
 constexpr int MT_MAX_N = 224;            // two accumulators of 224 columns and 64 columns of scales fill TMEM
-constexpr int MT_SMALL_N = 64;           // two of 64 columns and the scales half of it: two blocks per SM
+constexpr int MT_SMALL_N = 96;           // two of 96 columns and the scales half of it: two blocks per SM
 constexpr uint32_t MT_SF_STRIDE = 32, MT_SFB = 8;
 constexpr int MT_SFB_BYTES = 2048;
 constexpr int MT_MAX_STAGES = 8;
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         }
     } else if (warp == 8) {
         // ================= issuer =================
-        uint32_t s = 0, ph = 0, done = 0, par = 0;
+        uint32_t s = 0, ph = 0, done = 0, par = 0, ready = 0;
         bool ok = true;
         if (!a.c.offsets) {
             pdl_wait();
@@ -265,8 +265,11 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             const uint32_t id0 = mx_idesc(un.N, 0), id1 = mx_idesc(un.N, 1);
             const uint32_t d = tmem + buf * a.acc_cols;
             for (int kc = kc0; kc < kc1 && ok; kc++) {
-                ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
+                if (!ready) ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
                 if (!ok) break;
+                // the next stage's barriers are asked before this stage's MMAs go out: an answer takes some 130 cycles
+                const uint32_t ns = s + 1 == (uint32_t)a.stages ? 0 : s + 1, nph = ns ? ph : ph ^ 1u;
+                const uint32_t r_full = mbar_test(&bar_full[ns], nph), r_sf = mbar_test(&bar_sf[ns], nph);
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t st = stage0 + s * a.stage_bytes;
                 const uint32_t sf = tmem + 2 * a.acc_cols + par * MT_SF_STRIDE;
@@ -287,7 +290,9 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
                     if (kc == kc1 - 1) umma_commit(&bar_done[buf]);
                 }
                 __syncwarp();
-                if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
+                ready = __all_sync(0xffffffffu, r_full & r_sf);
+                s = ns;
+                ph = nph;
             }
             done++;
         }
@@ -428,21 +433,26 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         Unit un;
         if (first_unit < units && groups.unit(first_unit, &un)) {
             const int live = (a.w.chunks + a.share - 1) / a.share;
-            for (int i = rank * MT_THREADS + tid; i < un.n * (MX_TILE_ROWS / 2); i += a.split * MT_THREADS) {
-                const int n = i / (MX_TILE_ROWS / 2), p = i - n * (MX_TILE_ROWS / 2), m = un.tile * MX_TILE_ROWS + 2 * p;
-                if (m >= a.w.stored_rows) continue;
-                float2 v = make_float2(0.f, 0.f);
-                for (int k = 0; k < live; k++) {
-                    const float2 o = *(const float2*)(cluster.map_shared_rank((float*)stage_base, k) + n * MX_TILE_ROWS + 2 * p);
-                    v.x += o.x;
-                    v.y += o.y;
-                }
+            constexpr int PIECES = MX_TILE_ROWS / 4;     // four stored rows at a time; all blocks' parts are asked for at once
+            for (int i = rank * MT_THREADS + tid; i < un.n * PIECES; i += a.split * MT_THREADS) {
+                const int n = i / PIECES, p = i - n * PIECES, m = un.tile * MX_TILE_ROWS + 4 * p;
+                float4 o[MT_MAX_SPLIT];
+#pragma unroll
+                for (int k = 0; k < MT_MAX_SPLIT; k++)
+                    if (k < live) o[k] = *(const float4*)(cluster.map_shared_rank((float*)stage_base, k) + n * MX_TILE_ROWS + 4 * p);
+                float v[4] = {o[0].x, o[0].y, o[0].z, o[0].w};
+#pragma unroll
+                for (int k = 1; k < MT_MAX_SPLIT; k++)
+                    if (k < live) { v[0] += o[k].x; v[1] += o[k].y; v[2] += o[k].z; v[3] += o[k].w; }
                 T* y = (T*)a.c.y + (size_t)(un.row0 + n) * a.c.y_stride;
-                if (GATED) {
-                    y[m >> 1] = FloatType<FT>::down(gate_act(a.w.activation, v.x) * v.y);
-                } else {
-                    y[m] = FloatType<FT>::down(v.x);
-                    if (m + 1 < a.w.stored_rows) y[m + 1] = FloatType<FT>::down(v.y);
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    if (GATED) {
+                        if (m + j < a.w.stored_rows) y[(m + j) >> 1] = FloatType<FT>::down(gate_act(a.w.activation, v[j]) * v[j + 1]);
+                    } else {
+                        if (m + j < a.w.stored_rows) y[m + j] = FloatType<FT>::down(v[j]);
+                        if (m + j + 1 < a.w.stored_rows) y[m + j + 1] = FloatType<FT>::down(v[j + 1]);
+                    }
                 }
             }
         }
@@ -485,22 +495,40 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     MxTensorArgs a;
     a.w = w;
     a.c = c;
-    // Rows of a pass.  A dense product takes what it has; groups are seldom three times the average, and a pass more reads its
-    // weights again, from L2.  Fewer rows leave room for more stages.
-    const int expect = c.offsets ? std::min(c.rows, 3 * ((c.rows + w.experts - 1) / w.experts)) : c.rows;
+    // Rows of a pass.  A dense product takes what it has.  Groups: a quarter and 16 above the average; a longer group takes a pass
+    // more, which reads its weights again from L2.  Passes of up to 96 rows leave room for two blocks per SM (64 experts of
+    // 1536 x 5120, 16 / 31 / 63 rows on average: 58 / 89 / 93 us against 65 / 99 / 104 with one; at 125, in two passes each, 130
+    // against 111).
+    const int expect = c.offsets ? std::min(c.rows, (int)(1.25 * c.rows / w.experts) + 16) : c.rows;
     a.cap = std::min(MT_MAX_N, (expect + MT_BOX - 1) / MT_BOX * MT_BOX);
     a.stage_bytes = MX_TILE_BYTES + a.cap * MT_CHUNK + MT_SFB_BYTES;
     const bool small = a.cap <= MT_SMALL_N;
     a.acc_cols = small ? MT_SMALL_N : MT_MAX_N;
     a.tmem_cols = small ? 256 : 512;
-    a.stages = std::min(MT_MAX_STAGES, ((small ? MT_SMALL_SMEM : MT_SMEM) - 1024) / a.stage_bytes);
-    // Few units: a cluster shares one, a block at least two chunks
     const long long passes = c.offsets ? std::min<long long>(c.rows, c.rows / a.cap + w.experts) : (c.rows + a.cap - 1) / a.cap;
     const long long units = passes * w.row_tiles;
-    const int blocks = device_sms() * (small ? 2 : 1);
+    // Few units: a cluster shares each.  Joining the parts costs about as much as four to six chunks of one block (0.33 us each):
+    // 4096 x 4096, one row: 8.3 / 6.9 / 6.8 us by clusters of 1 / 2 / 4; 5120 x 1536, 32 rows: 4.8 / 6.4.  Blocks that wait for a
+    // place cost more than they save: 96 units of 20 chunks 13.1 / 13.8 / 19.6.  Clusters of blocks that fill an SM each do not
+    // cover all SMs (17 of eight blocks: 11.9 us against 6.2 for 17 of four).
+    const int sms = device_sms(), places = small ? sms + sms / 12 : sms - sms / 8;
     a.split = 1;
-    while (a.split < MT_MAX_SPLIT && units * a.split * 2 <= blocks && a.split * 4 <= w.chunks) a.split *= 2;
-    a.share = (w.chunks + a.split - 1) / a.split;
+    a.share = w.chunks;
+    int cost = w.chunks;
+    for (int split = 2; split <= MT_MAX_SPLIT && units * split <= places; split *= 2) {
+        const int share = (w.chunks + split - 1) / split;
+        if (share + 4 + split / 4 < cost) {
+            a.split = split;
+            a.share = share;
+            cost = share + 4 + split / 4;
+        }
+    }
+    // Two blocks per SM where there is work for them or where half the stages hold all chunks; otherwise one with twice the stages
+    const int half = std::min(MT_MAX_STAGES, (MT_SMALL_SMEM - 1024) / a.stage_bytes);
+    const bool pairs = small && (units * a.split > sms || a.share <= half);
+    const int blocks = pairs ? 2 * sms : sms;
+    a.stages = std::min(a.share, pairs ? half : std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes));
+    if (a.split > 1) a.stages = std::max(a.stages, (a.cap * MX_TILE_ROWS * 4 + a.stage_bytes - 1) / a.stage_bytes);    // partial sums
     const size_t smem = (size_t)a.stages * a.stage_bytes + 1024;
     const int grid = a.split > 1 ? (int)units * a.split : (int)std::min<long long>(blocks, units);
     const auto kernel = w.activation ? (c.y_type == FT_F32    ? mxfp4_tensor_kernel<FT_F32, true>

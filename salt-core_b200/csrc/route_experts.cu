@@ -15,6 +15,8 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <limits.h>
+
 #include <algorithm>
 
 #include "../../include/salt_gpu_b200.h"
@@ -31,8 +33,10 @@ namespace {
 
 constexpr int RT_WARPS = 4;              // tokens of a block of the routing kernel
 constexpr int RT_FUSED_TOKENS = 16;      // up to here one block routes and groups
-constexpr int GR_WARPS = 16;
+constexpr int GR_WARPS = 32;
+constexpr int GR_HELD = 8;               // selections of a lane that stay in registers between the two passes
 constexpr int GR_CLUSTER = 8;
+constexpr int GR_FEW = 512;              // RT_FUSED_TOKENS times the largest top-k
 constexpr int GR_ONE_BLOCK = 2048;       // selections that one block groups by itself
 constexpr unsigned FULL = 0xffffffffu;
 
@@ -63,6 +67,7 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 template <typename S> struct Keys;
 template <> struct Keys<float> {
     using K = uint32_t;
+    static __device__ __forceinline__ float quotient(float a, float b) { return __fdividef(a, b); }     // 2 units
     static __device__ __forceinline__ K of(float v) { return v > -CUDART_INF_F ? ordered(v) : 0u; }     // false for NaN
     static __device__ __forceinline__ float value(K k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
     static __device__ __forceinline__ K best(K k, int e, int& at) {
@@ -73,6 +78,7 @@ template <> struct Keys<float> {
 };
 template <> struct Keys<double> {
     using K = unsigned long long;
+    static __device__ __forceinline__ double quotient(double a, double b) { return a / b; }
     static __device__ __forceinline__ K of(double v) {
         if (!(v > -CUDART_INF)) return 0ull;
         const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
@@ -113,7 +119,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         for (int i = 0; i < VPT; i++) {
             const S x = (S)l[i];
             const S t = exp(x < (S)0 ? x : -x);          // at most 1
-            score[i] = (x < (S)0 ? t : (S)1) / ((S)1 + t);
+            score[i] = Q::quotient(x < (S)0 ? t : (S)1, (S)1 + t);
         }
     } else {
         float m = -CUDART_INF_F;
@@ -131,7 +137,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         if (sum > (S)0) {
             top_score = (S)1 / sum;
 #pragma unroll
-            for (int i = 0; i < VPT; i++) score[i] = score[i] / sum;
+            for (int i = 0; i < VPT; i++) score[i] = wide ? score[i] / sum : score[i] * top_score;
         }
     }
     K key[VPT];                                          // 0: this expert cannot be chosen
@@ -163,13 +169,13 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         if (g < a.groups)
             for (int j = sub; j < per; j += share) {
                 const K k = keys[g * per + j];
-                if (k > k1) { k2 = k1; k1 = k; }
-                else if (k > k2) k2 = k;
+                k2 = max(k2, min(k1, k));
+                k1 = max(k1, k);
             }
         for (int d = 1; d < share; d <<= 1) {
             const K o1 = __shfl_xor_sync(FULL, k1, d), o2 = __shfl_xor_sync(FULL, k2, d);
-            if (o1 > k1) { k2 = max(k1, o2); k1 = o1; }
-            else k2 = max(k2, o1);
+            k2 = max(max(k2, o2), min(k1, o1));
+            k1 = max(k1, o1);
         }
         __syncwarp();
         K mine = k1;
@@ -280,28 +286,49 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     uint32_t* total = hist + warps * a.E;                // this block's selections of every expert
     uint32_t* base = total + a.E;                        // where this block's part of the group begins
-    for (int i = tid; i < warps * a.E; i += blockDim.x) hist[i] = 0;
-    __syncthreads();
     const int piece = ((a.n + warps * blocks - 1) / (warps * blocks) + 31) & ~31;
     const int w_all = rank * warps + warp;
     const int begin = (int)min((long long)w_all * piece, (long long)a.n);
     const int end = (int)min((long long)begin + piece, (long long)a.n);
+    int held[GR_HELD];
+#pragma unroll
+    for (int j = 0; j < GR_HELD; j++) {
+        const int i = begin + 32 * j + lane;
+        held[j] = i < end ? a.selected[i] : -1;
+    }
+    for (int i = tid; i < warps * a.E; i += blockDim.x) hist[i] = 0;
+    __syncthreads();
     uint32_t* mine = hist + warp * a.E;
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < end ? a.selected[i] : -1;
-        const bool ok = e >= 0 && e < a.E;
-        const uint32_t same = __match_any_sync(FULL, ok ? e : -1);
-        if (ok && lane == __ffs(same) - 1) mine[e] += __popc(same);
-        __syncwarp();
+    for (int i0 = begin; i0 < end; i0 += 32 * GR_HELD) {
+        if (i0 > begin) {
+#pragma unroll
+            for (int j = 0; j < GR_HELD; j++) {
+                const int i = i0 + 32 * j + lane;
+                held[j] = i < end ? a.selected[i] : -1;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < GR_HELD; j++) {
+            if (i0 + 32 * j >= end) break;
+            const int e = held[j];
+            const bool ok = e >= 0 && e < a.E;
+            const uint32_t same = __match_any_sync(FULL, ok ? e : -1);
+            if (ok && lane == __ffs(same) - 1) mine[e] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
     for (int e = tid; e < a.E; e += blockDim.x) {        // prefix over the warps
         uint32_t t = 0;
-        for (int w = 0; w < warps; w++) {
-            const uint32_t c = hist[w * a.E + e];
-            hist[w * a.E + e] = t;
-            t += c;
+        for (int w0 = 0; w0 < warps; w0 += 8) {
+            uint32_t c[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) c[j] = hist[(w0 + j) * a.E + e];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                hist[(w0 + j) * a.E + e] = t;
+                t += c[j];
+            }
         }
         total[e] = t;
     }
@@ -315,7 +342,8 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
         if (e >= a.E) break;
         uint32_t all = 0, before = 0;
         if (cluster) {
-            for (int b = 0; b < blocks; b++) {
+#pragma unroll
+            for (int b = 0; b < GR_CLUSTER; b++) {
                 const uint32_t c = *cg::this_cluster().map_shared_rank(total + e, b);
                 if (b < rank) before += c;
                 all += c;
@@ -356,22 +384,32 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
         for (int e = tid; e < a.E; e += blockDim.x) a.offsets[e] = (int32_t)base[e];
         if (tid == 0) a.offsets[a.E] = (int32_t)s_live;
     }
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < end ? a.selected[i] : -1;
-        const bool ok = e >= 0 && e < a.E;
-        const uint32_t same = __match_any_sync(FULL, ok ? e : -1);
-        uint32_t p = 0;
-        if (ok) p = base[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
-        __syncwarp();
-        if (ok) {
-            a.g2c[p] = i;
-            a.c2g[i] = (int32_t)p;
-            if (lane == __ffs(same) - 1) mine[e] += __popc(same);
-        } else if (i < end) {
-            a.c2g[i] = -1;
+    for (int i0 = begin; i0 < end; i0 += 32 * GR_HELD) {
+        if (piece > 32 * GR_HELD) {
+#pragma unroll
+            for (int j = 0; j < GR_HELD; j++) {
+                const int i = i0 + 32 * j + lane;
+                held[j] = i < end ? a.selected[i] : -1;
+            }
         }
-        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < GR_HELD; j++) {
+            if (i0 + 32 * j >= end) break;
+            const int i = i0 + 32 * j + lane, e = held[j];
+            const bool ok = e >= 0 && e < a.E;
+            const uint32_t same = __match_any_sync(FULL, ok ? e : -1);
+            uint32_t p = 0;
+            if (ok) p = base[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
+            __syncwarp();
+            if (ok) {
+                a.g2c[p] = i;
+                a.c2g[i] = (int32_t)p;
+                if (lane == __ffs(same) - 1) mine[e] += __popc(same);
+            } else if (i < end) {
+                a.c2g[i] = -1;
+            }
+            __syncwarp();
+        }
     }
     for (long long p = (long long)s_live + (long long)rank * blockDim.x + tid; p < a.n; p += (long long)blocks * blockDim.x)
         a.g2c[p] = -1;
@@ -400,23 +438,47 @@ __global__ void __launch_bounds__(GR_WARPS * 32) group_kernel(const GroupArgs a)
     group_selections(a, (uint32_t*)smem, (int)blockIdx.x, (int)gridDim.x, cluster);
 }
 
+// Up to 512 selections: a thread per selection, and per expert, counts the selections that come before it.
+__device__ void group_few(const GroupArgs& a) {
+    __shared__ int s_sel[GR_FEW];
+    const int tid = threadIdx.x;
+    for (int i = tid; i < a.n; i += blockDim.x) {
+        const int e = a.selected[i];
+        s_sel[i] = e >= 0 && e < a.E ? e : INT_MAX;      // behind every group
+    }
+    __syncthreads();
+    for (int i = tid; i < a.n; i += blockDim.x) {
+        const int e = s_sel[i];
+        int p = 0;
+        for (int j = 0; j < a.n; j++) p += s_sel[j] < e || (s_sel[j] == e && j < i);
+        a.c2g[i] = e == INT_MAX ? -1 : p;
+        a.g2c[p] = e == INT_MAX ? -1 : i;
+    }
+    for (int e = tid; e <= a.E; e += blockDim.x) {
+        int p = 0;
+        for (int j = 0; j < a.n; j++) p += s_sel[j] < e;
+        a.offsets[e] = p;
+    }
+}
+
 // Few tokens: one block routes them, a warp each, and groups what they selected.
-template <int VPT> __global__ void __launch_bounds__(GR_WARPS * 32) route_group_kernel(const RouteArgs a, const GroupArgs g) {
+template <int VPT> __global__ void __launch_bounds__(RT_FUSED_TOKENS * 32) route_group_kernel(const RouteArgs a, const GroupArgs g) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
     pdl_launch_dependents();
     if (warp < a.rows) route_row<VPT>(a, warp, lane, smem + route_smem(a.E, a.groups, warp));
     __syncthreads();
-    group_selections(g, (uint32_t*)smem, 0, 1, false);
+    group_few(g);
 }
 
 template <int VPT> cudaError_t launch_route(const RouteArgs& a, const GroupArgs* g, cudaStream_t stream) {
     cudaError_t e;
     if (g && a.rows <= RT_FUSED_TOKENS && a.rows > 0) {
-        const size_t smem = std::max(group_smem(a.E, GR_WARPS), route_smem(a.E, a.groups, RT_FUSED_TOKENS));
+        const int warps = std::max(a.rows, 4);           // a warp per token; four at least, for the counting
+        const size_t smem = route_smem(a.E, a.groups, a.rows);
         if (smem > PLAIN_DYNAMIC_SMEM && (e = ensure_dynamic_smem((const void*)route_group_kernel<VPT>, smem)) != cudaSuccess) return e;
-        return launch_pdl(route_group_kernel<VPT>, dim3(1), dim3(GR_WARPS * 32), smem, stream, a, *g);
+        return launch_pdl(route_group_kernel<VPT>, dim3(1), dim3(warps * 32), smem, stream, a, *g);
     }
     if (a.rows > 0) {
         const size_t smem = route_smem(a.E, a.groups, RT_WARPS);
