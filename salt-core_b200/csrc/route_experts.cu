@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t ordered(float v) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// Keys as they are compared: in 32 bits by two integer reductions, in 64 by exchanging pairs.
+// Keys as they are compared, by integer reductions over the warp: the largest key and its lowest index.
 template <typename S> struct Keys;
 template <> struct Keys<float> {
     using K = uint32_t;
@@ -88,14 +88,11 @@ template <> struct Keys<double> {
         return __longlong_as_double((long long)((k >> 63) ? (k & 0x7fffffffffffffffull) : ~k));
     }
     static __device__ __forceinline__ K best(K k, int e, int& at) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            const K ok = __shfl_xor_sync(FULL, k, d);
-            const int oe = __shfl_xor_sync(FULL, e, d);
-            if (ok > k || (ok == k && oe < e)) { k = ok; e = oe; }
-        }
-        at = e;
-        return k;
+        const unsigned hi = __reduce_max_sync(FULL, (unsigned)(k >> 32));
+        const unsigned lo = __reduce_max_sync(FULL, (unsigned)(k >> 32) == hi ? (unsigned)k : 0u);
+        const K m = ((K)hi << 32) | lo;
+        at = (int)__reduce_min_sync(FULL, k == m ? (unsigned)e : 0x7fffffffu);
+        return m;
     }
 };
 
@@ -148,9 +145,10 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         if (a.bias) key[i] = live ? Q::of(score[i] + (S)__ldg(a.bias + min(e, a.E - 1))) : 0;
         else key[i] = live ? Q::of((S)l[i]) : 0;
     }
-    // Rounding errors of two keys together: a score is off by less than 2e-6 of the largest (its exponential by two units of
-    // the last place, the difference before it by |l - m| / 2 units, the sum by 37 additions), the bias adds one rounding.
-    const S slack = wide ? (S)0 : (S)4e-6 * top_score;
+    // Rounding errors of two keys together.  Softmax: a score is off by less than 2e-6 of the largest (its exponential by two units
+    // of the last place, the difference before it by |l - m| / 2 units, the sum by 37 additions).  Sigmoid: by 4.2e-7 (exponential
+    // and quotient two units each, the sum half a unit).  The bias adds one rounding, below.
+    const S slack = wide ? (S)0 : a.sigmoid ? (S)1e-6 : (S)4e-6 * top_score;
     if (a.groups > 1) {
         K* keys = (K*)sh;
         const int per = a.E / a.groups;
@@ -281,22 +279,37 @@ template <int VPT> __device__ __forceinline__ void route_row(const RouteArgs& a,
 // Stable counting sort of the selections by expert.  A warp owns a contiguous piece of them and a histogram; the pieces of a
 // block's warps, and of a cluster's blocks, follow one another, so positions keep the canonical order inside an expert.
 // Selections outside [0, E) belong to no group: their place is -1, and so are the entries behind the last group.
+// The lanes of a warp that hold the same expert find one another by setting their bits in a word per expert (the instruction that
+// compares all lanes takes 270 cycles a warp where the experts differ: 16.5 us for 32792 selections).
+__device__ __forceinline__ uint32_t same_expert(uint32_t* bits, int e, bool ok, int lane) {
+    if (ok) atomicOr(bits + e, 1u << lane);
+    __syncwarp();
+    const uint32_t same = ok ? bits[e] : 0u;
+    __syncwarp();
+    if (ok) bits[e] = 0;
+    return same;                                         // the caller's next __syncwarp lets the words be set again
+}
+
 __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, int blocks, bool cluster) {
     __shared__ uint32_t s_part[32], s_live;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
-    uint32_t* total = hist + warps * a.E;                // this block's selections of every expert
+    uint32_t* bits = hist + (warps + warp) * a.E;        // this warp's words
+    uint32_t* total = hist + 2 * warps * a.E;            // this block's selections of every expert
     uint32_t* base = total + a.E;                        // where this block's part of the group begins
     const int piece = ((a.n + warps * blocks - 1) / (warps * blocks) + 31) & ~31;
     const int w_all = rank * warps + warp;
     const int begin = (int)min((long long)w_all * piece, (long long)a.n);
     const int end = (int)min((long long)begin + piece, (long long)a.n);
+    const bool keep = piece <= 32 * GR_HELD;
     int held[GR_HELD];
+    uint32_t same[GR_HELD];
 #pragma unroll
     for (int j = 0; j < GR_HELD; j++) {
         const int i = begin + 32 * j + lane;
         held[j] = i < end ? a.selected[i] : -1;
+        same[j] = 0;
     }
-    for (int i = tid; i < warps * a.E; i += blockDim.x) hist[i] = 0;
+    for (int i = tid; i < 2 * warps * a.E; i += blockDim.x) hist[i] = 0;
     __syncthreads();
     uint32_t* mine = hist + warp * a.E;
     for (int i0 = begin; i0 < end; i0 += 32 * GR_HELD) {
@@ -312,8 +325,8 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
             if (i0 + 32 * j >= end) break;
             const int e = held[j];
             const bool ok = e >= 0 && e < a.E;
-            const uint32_t same = __match_any_sync(FULL, ok ? e : -1);
-            if (ok && lane == __ffs(same) - 1) mine[e] += __popc(same);
+            same[j] = same_expert(bits, e, ok, lane);
+            if (ok && lane == __ffs(same[j]) - 1) mine[e] += __popc(same[j]);
             __syncwarp();
         }
     }
@@ -385,7 +398,7 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
         if (tid == 0) a.offsets[a.E] = (int32_t)s_live;
     }
     for (int i0 = begin; i0 < end; i0 += 32 * GR_HELD) {
-        if (piece > 32 * GR_HELD) {
+        if (!keep) {
 #pragma unroll
             for (int j = 0; j < GR_HELD; j++) {
                 const int i = i0 + 32 * j + lane;
@@ -397,14 +410,14 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
             if (i0 + 32 * j >= end) break;
             const int i = i0 + 32 * j + lane, e = held[j];
             const bool ok = e >= 0 && e < a.E;
-            const uint32_t same = __match_any_sync(FULL, ok ? e : -1);
+            const uint32_t lanes = keep ? same[j] : same_expert(bits, e, ok, lane);
             uint32_t p = 0;
-            if (ok) p = base[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
+            if (ok) p = base[e] + mine[e] + __popc(lanes & ((1u << lane) - 1u));
             __syncwarp();
             if (ok) {
                 a.g2c[p] = i;
                 a.c2g[i] = (int32_t)p;
-                if (lane == __ffs(same) - 1) mine[e] += __popc(same);
+                if (lane == __ffs(lanes) - 1) mine[e] += __popc(lanes);
             } else if (i < end) {
                 a.c2g[i] = -1;
             }
@@ -416,7 +429,7 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
     if (cluster) cg::this_cluster().sync();              // a block's totals are read by the others until here
 }
 
-__host__ __device__ inline size_t group_smem(int E, int warps) { return (size_t)(warps + 2) * E * sizeof(uint32_t); }
+__host__ __device__ inline size_t group_smem(int E, int warps) { return (size_t)(2 * warps + 2) * E * sizeof(uint32_t); }
 __host__ __device__ inline size_t route_smem(int E, int groups, int warps) {
     return groups > 1 ? (size_t)warps * E * sizeof(unsigned long long) : 0;
 }
@@ -486,10 +499,11 @@ template <int VPT> cudaError_t launch_route(const RouteArgs& a, const GroupArgs*
         if (e != cudaSuccess) return e;
     }
     if (!g) return cudaSuccess;
-    const size_t smem = group_smem(a.E, GR_WARPS);
+    const int warps = a.E <= 512 ? GR_WARPS : GR_WARPS / 2;          // two words per expert and warp: at most 139 KB
+    const size_t smem = group_smem(a.E, warps);
     if (smem > PLAIN_DYNAMIC_SMEM && (e = ensure_dynamic_smem((const void*)group_kernel, smem)) != cudaSuccess) return e;
-    if (g->n > GR_ONE_BLOCK) return launch_pdl_cluster(group_kernel, GR_CLUSTER, dim3(GR_WARPS * 32), smem, stream, *g);
-    return launch_pdl(group_kernel, dim3(1), dim3(GR_WARPS * 32), smem, stream, *g);
+    if (g->n > GR_ONE_BLOCK) return launch_pdl_cluster(group_kernel, GR_CLUSTER, dim3(warps * 32), smem, stream, *g);
+    return launch_pdl(group_kernel, dim3(1), dim3(warps * 32), smem, stream, *g);
 }
 
 }  // namespace
