@@ -33,6 +33,55 @@ struct QuantArgs {
     void* values;
 };
 
+// Eight columns as they were loaded.  The largest magnitude is found on the bits (NaN lies above infinity), of 16-bit types two at a
+// time, and returned as the bits of a float.
+template <int FT> struct Raw8 {
+    using T = typename FloatType<FT>::T;
+    uint4 q = make_uint4(0, 0, 0, 0);
+    __device__ __forceinline__ void load(const T* p) { q = *(const uint4*)p; }
+    __device__ __forceinline__ uint32_t top_of_four_lanes() const {
+        constexpr uint32_t M = 0x7fff7fffu;
+        uint32_t t = __vmaxu2(__vmaxu2(q.x & M, q.y & M), __vmaxu2(q.z & M, q.w & M));
+        t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = __vmaxu2(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        t = max(t & 0xffffu, t >> 16);
+        if (FT == FT_BF16) return t << 16;
+        const __half_raw h = {(unsigned short)t};
+        return __float_as_uint(__half2float(__half(h)));
+    }
+    __device__ __forceinline__ void floats(float (&f)[8]) const {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (FT == FT_BF16) {
+                f[2 * i] = __uint_as_float(w[i] << 16);
+                f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            } else {
+                const float2 p = __half22float2(*(const __half2*)&w[i]);
+                f[2 * i] = p.x;
+                f[2 * i + 1] = p.y;
+            }
+        }
+    }
+};
+template <> struct Raw8<FT_F32> {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    __device__ __forceinline__ void load(const float* p) { a = ((const float4*)p)[0]; b = ((const float4*)p)[1]; }
+    __device__ __forceinline__ void floats(float (&f)[8]) const {
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    }
+    __device__ __forceinline__ uint32_t top_of_four_lanes() const {
+        float f[8];
+        floats(f);
+        uint32_t t = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) t = max(t, __float_as_uint(f[i]) & 0x7fffffffu);
+        t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        return max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+    }
+};
+
 // A block works on one row, a thread on U pieces of eight columns, whose loads are all in flight before the first is used.
 template <int FT, bool VALUES, int U> __global__ void __launch_bounds__(MQ_MAX_THREADS) mxfp4_quantize_kernel(const QuantArgs a) {
     using T = typename FloatType<FT>::T;
@@ -41,44 +90,40 @@ template <int FT, bool VALUES, int U> __global__ void __launch_bounds__(MQ_MAX_T
     const int row = blockIdx.x;
     int src = row;
     if (a.index) {
-        src = __ldg(a.index + row);
+        src = a.index[row];
         if (src < 0) return;                             // an index below zero leaves its row as it was
         src = (int)((unsigned)src / (unsigned)a.div);
     }
     if (src >= a.src_rows) return;
     const T* x = (const T*)a.x + (size_t)src * a.stride;
     const int first = blockIdx.y * U * blockDim.x + threadIdx.x, units = a.cols / 8;
-    float v[U][8];
+    Raw8<FT> v[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int unit = first + u * blockDim.x;         // the four lanes of a block of 32 columns agree on it
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[u][i] = 0.f;
-        if (unit < units) load8<FT>(x + unit * 8, v[u]);
+        if (unit < units) v[u].load(x + unit * 8);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int unit = first + u * blockDim.x;
-        uint32_t top = 0;                                // magnitudes order like their bits, NaN above infinity
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[u][i]) & 0x7fffffffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const uint32_t top = v[u].top_of_four_lanes();
         const uint32_t ex = top >> 23;                   // biased exponent; 0: subnormal or zero
         const bool bad = ex == 255u;
         const uint32_t s = bad ? 255u : (ex > 2u ? ex - 2u : 0u);
         const float up = __uint_as_float((254u - min(s, 253u)) << 23);   // 2^(127 - s); s is at most 252 unless bad
-        uint32_t packed = 0;
+        float f[8];
+        v[u].floats(f);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            uint32_t b;
-            asm("{ .reg .b8 q;\n\t"
-                "cvt.rn.satfinite.e2m1x2.f32 q, %2, %1;\n\t"
-                "cvt.u32.u8 %0, q; }\n"
-                : "=r"(b)
-                : "f"(__fmul_rn(v[u][2 * i], up)), "f"(__fmul_rn(v[u][2 * i + 1], up)));
-            packed |= b << (8 * i);
-        }
+        for (int i = 0; i < 8; i++) f[i] = __fmul_rn(f[i], up);
+        uint32_t packed;
+        asm("{ .reg .b8 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+            "mov.b32 %0, {a, b, c, d}; }\n"
+            : "=r"(packed)
+            : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
         if (bad) packed = 0;
         if (unit >= units) continue;
         *(uint32_t*)(a.codes + (size_t)row * (a.cols / 2) + unit * 4) = packed;

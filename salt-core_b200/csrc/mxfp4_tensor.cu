@@ -9,8 +9,7 @@
 // Warp roles:
 //   warp 9      producer: one bulk copy of the weight tile, codes and scales, which lies in memory as the tensor core reads it, and
 //               TMA copies of the rows' codes (boxes of 32 rows, 128-byte swizzle)
-//   warps 0-3   scales of the rows: 16 bytes per row and pair of chunks, loaded a pair ahead, written to shared memory in the order
-//               of a scale tile
+//   warps 0-3   scales of the rows: a chunk each in turn, loaded a turn ahead, written to shared memory in the order of a scale tile
 //   warp 8      issuer: tcgen05.cp of the chunk's scale tiles to TMEM, then its four MMAs; both run in issue order
 //   warps 4-7   epilogue: lane = weight row, column = row of the result; a gated pair's two rows are neighbouring lanes
 // Every mbarrier wait is bounded; on expiry the block raises its failure flag, sets SB_ERR_TIMEOUT, waits (bounded) for copies
@@ -52,25 +51,55 @@ struct MxTensorArgs {
 };
 
 // kind::mxf4 instruction descriptor: A = B = E2M1, K-major, E8M0 scales, `half` = which two bytes of a scale word the MMA reads.
-__device__ __forceinline__ uint32_t mx_idesc(int N, uint32_t half) {
-    return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | (1u << 27) | (half << 5) | (half << 30);
+__device__ __forceinline__ uint32_t mx_idesc(int M, int N, uint32_t half) {
+    return (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | (half << 5) | (half << 30);
 }
 
+// PAIR: the instruction works on both SMs of a pair; all tcgen05 instructions of a kernel are of one kind.
+template <bool PAIR>
 __device__ __forceinline__ void mx_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// 32 rows of 16 bytes, unswizzled (8-row groups 128 bytes apart), to four TMEM columns of all four lane quarters; of a pair, each
+// SM from its own shared memory.
+template <bool PAIR> __device__ __forceinline__ void scale_copy(uint32_t taddr, uint32_t smem) {
+    const uint64_t desc = make_desc((smem & 0x3ffffu) >> 4, (128u >> 4) | (1u << 14));
+    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Arrival at a barrier once everything issued so far is complete; of a pair, at the barriers of both blocks.
+template <bool PAIR> __device__ __forceinline__ void mx_commit(uint64_t* bar) {
+    if constexpr (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else umma_commit(bar);
+}
+
+// Arrival at the same barrier of another block of the cluster.
+__device__ __forceinline__ void remote_arrive(uint64_t* bar, uint32_t rank) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "{\n\t.reg .b32 r;\n\t"
+        "mapa.shared::cluster.u32 r, %0, %1;\n\t"
+        "mbarrier.arrive.shared::cluster.b64 _, [r];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(rank)
         : "memory");
 }
-
-// 32 rows of 16 bytes, unswizzled (8-row groups 128 bytes apart), to four TMEM columns of all four lane quarters.
-__device__ __forceinline__ void scale_copy(uint32_t taddr, uint32_t smem) {
-    const uint64_t desc = make_desc((smem & 0x3ffffu) >> 4, (128u >> 4) | (1u << 14));
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
 // One lane of a converged warp.  The instructions for copies and MMAs take their operands from the warp's uniform registers: inside
 // this election, with operands that are the same in all lanes, they are issued at once; under `lane == 0` the compiler has to
 // go through the lanes, and a chunk's four MMAs, six scale copies and commit took 1100 cycles.
@@ -125,11 +154,11 @@ struct Groups {
     }
 };
 
-template <int FT, bool GATED>
+template <int FT, bool GATED, bool PAIR>
 __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTensorArgs a, const __grid_constant__ CUtensorMap xmap) {
     using T = typename FloatType<FT>::T;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bar_free[MT_MAX_STAGES], bar_full[MT_MAX_STAGES], bar_sf[MT_MAX_STAGES];
+    __shared__ __align__(8) uint64_t bar_free[MT_MAX_STAGES], bar_full[MT_MAX_STAGES], bar_sf[MT_MAX_STAGES], bar_peer[MT_MAX_STAGES];
     __shared__ __align__(8) uint64_t bar_done[2], bar_accfree[2], bar_drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail;
@@ -143,20 +172,27 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         for (int s = 0; s < a.stages; s++) {
             mbar_init(&bar_free[s], 1);
             mbar_init(&bar_full[s], 1);
-            mbar_init(&bar_sf[s], 4);
+            mbar_init(&bar_sf[s], 1);
+            mbar_init(&bar_peer[s], 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&bar_done[b], 1);
-            mbar_init(&bar_accfree[b], 4);
+            mbar_init(&bar_accfree[b], PAIR ? 8 : 4);
         }
         mbar_init(&bar_drain, 1);
         s_fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(a.tmem_cols)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(a.tmem_cols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(a.tmem_cols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     // A dense product's weights do not wait for the launch before: the producer asks for them first.
     if (a.c.offsets) {
@@ -195,16 +231,19 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         if (tid == MT_THREADS - 1) s_first[a.w.experts] = front + sum;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if (PAIR) cg::this_cluster().sync();                 // the other block's barriers and TMEM are there
+    else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = (uint32_t)uniform((int)s_tmem);
     Groups groups;
     groups.first = a.c.offsets ? s_first : nullptr;
-    groups.begin = s_begin; groups.experts = a.w.experts; groups.rows = a.c.rows; groups.cap = a.cap; groups.tiles = a.w.row_tiles;
+    groups.begin = s_begin; groups.experts = a.w.experts; groups.rows = a.c.rows; groups.cap = a.cap;
+    groups.tiles = PAIR ? (a.w.row_tiles + 1) / 2 : a.w.row_tiles;   // of a pair, a unit is two tiles
     const int size = pass_rows(a.c.rows, a.cap);
-    const int units = (a.c.offsets ? s_first[a.w.experts] : (a.c.rows + size - 1) / size) * a.w.row_tiles;
-    const int rank = a.split > 1 ? (int)(blockIdx.x % a.split) : 0, first_unit = (int)blockIdx.x / a.split, unit_step = (int)gridDim.x / a.split;
-    const int kc0 = rank * a.share, kc1 = min(a.w.chunks, kc0 + a.share);
+    const int units = (a.c.offsets ? s_first[a.w.experts] : (a.c.rows + size - 1) / size) * groups.tiles;
+    const int cluster_size = PAIR ? 2 : a.split;
+    const int rank = (int)(blockIdx.x % cluster_size), first_unit = (int)blockIdx.x / cluster_size, unit_step = (int)gridDim.x / cluster_size;
+    const int kc0 = PAIR ? 0 : rank * a.share, kc1 = PAIR ? a.w.chunks : min(a.w.chunks, kc0 + a.share);
     const int sfb_off = a.stage_bytes - MT_SFB_BYTES;    // a stage: weight tile, rows' codes, rows' scales
 
     const uint32_t stage0 = (uint32_t)uniform((int)smem_u32(stage_base));
@@ -216,9 +255,12 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         for (int u = first_unit; u < units && ok; u += unit_step) {
             Unit un;
             if (!groups.unit_uniform(u, &un)) continue;
-            const int boxes = (un.N + MT_BOX - 1) / MT_BOX;
+            // of a pair, each block brings its own tile (the last one twice where they are odd) and half of the rows
+            const int half = PAIR ? un.N / 2 : un.N, row0 = un.row0 + (PAIR ? rank * half : 0);
+            const int boxes = (half + MT_BOX - 1) / MT_BOX;
             const uint32_t tx = MX_TILE_BYTES + boxes * (MT_BOX * MT_CHUNK);
-            const uint8_t* tile = a.w.tiles + ((size_t)un.expert * a.w.row_tiles + un.tile) * a.w.chunks * MX_TILE_BYTES;
+            const int tile_at = PAIR ? min(2 * un.tile + rank, a.w.row_tiles - 1) : un.tile;
+            const uint8_t* tile = a.w.tiles + ((size_t)un.expert * a.w.row_tiles + tile_at) * a.w.chunks * MX_TILE_BYTES;
             int early = kc0;                             // weights of the chunks below have been asked for
             if (!waited) {
                 early = min(kc1, kc0 + a.stages);
@@ -243,8 +285,26 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
                         bulk_load(dst, tile + (size_t)kc * MX_TILE_BYTES, MX_TILE_BYTES, smem_u32(&bar_full[s]));
                     }
                     for (int b = 0; b < boxes; b++)
-                        tma_load_2d(dst + MX_TILE_BYTES + b * (MT_BOX * MT_CHUNK), &xmap, kc * MT_CHUNK, un.row0 + b * MT_BOX, &bar_full[s]);
+                        tma_load_2d(dst + MX_TILE_BYTES + b * (MT_BOX * MT_CHUNK), &xmap, kc * MT_CHUNK, row0 + b * MT_BOX, &bar_full[s]);
                 }
+                __syncwarp();
+                if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (PAIR && warp == 8 && rank == 1) {
+        // ================= second block of a pair: its stages, reported to the first =================
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        if (!a.c.offsets) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
+        for (int u = first_unit; u < units && ok; u += unit_step) {
+            Unit un;
+            if (!groups.unit_uniform(u, &un)) continue;
+            for (int kc = kc0; kc < kc1 && ok; kc++) {
+                ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
+                if (ok && lane == 0) remote_arrive(&bar_peer[s], 0);
                 __syncwarp();
                 if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
             }
@@ -261,15 +321,17 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             Unit un;
             if (!groups.unit_uniform(u, &un)) continue;
             const uint32_t buf = done & 1u;
-            if (done >= 2u) ok = __all_sync(0xffffffffu, mbar_wait(&bar_accfree[buf], ((done >> 1) - 1) & 1, fail));
-            const uint32_t id0 = mx_idesc(un.N, 0), id1 = mx_idesc(un.N, 1);
+            if (done >= 2u)
+                ok = __all_sync(0xffffffffu, mbar_wait(&bar_accfree[buf], ((done >> 1) - 1) & 1, fail));
+            const uint32_t id0 = mx_idesc(PAIR ? 256 : 128, un.N, 0), id1 = mx_idesc(PAIR ? 256 : 128, un.N, 1);
             const uint32_t d = tmem + buf * a.acc_cols;
             for (int kc = kc0; kc < kc1 && ok; kc++) {
                 if (!ready) ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
+                if (PAIR && !ready && ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar_peer[s], ph, fail));
                 if (!ok) break;
                 // the next stage's barriers are asked before this stage's MMAs go out: an answer takes some 130 cycles
                 const uint32_t ns = s + 1 == (uint32_t)a.stages ? 0 : s + 1, nph = ns ? ph : ph ^ 1u;
-                const uint32_t r_full = mbar_test(&bar_full[ns], nph), r_sf = mbar_test(&bar_sf[ns], nph);
+                const uint32_t r_full = mbar_test(&bar_full[ns], nph), r_sf = mbar_test(&bar_sf[ns], nph), r_peer = PAIR ? mbar_test(&bar_peer[ns], nph) : 1u;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t st = stage0 + s * a.stage_bytes;
                 const uint32_t sf = tmem + 2 * a.acc_cols + par * MT_SF_STRIDE;
@@ -277,20 +339,20 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
                 if (elected()) {
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        scale_copy(sf + 4 * k, st + MX_CODE_BYTES + k * 512);
-                        scale_copy(sf + MT_SFB + 8 * k, st + sfb_off + k * 1024);
-                        if (un.N > 128) scale_copy(sf + MT_SFB + 8 * k + 4, st + sfb_off + k * 1024 + 512);
+                        scale_copy<PAIR>(sf + 4 * k, st + MX_CODE_BYTES + k * 512);
+                        scale_copy<PAIR>(sf + MT_SFB + 8 * k, st + sfb_off + k * 1024);
+                        if (un.N > 128) scale_copy<PAIR>(sf + MT_SFB + 8 * k + 4, st + sfb_off + k * 1024 + 512);
                     }
                     const uint32_t alo = DESC_B_LO | ((st & 0x3ffffu) >> 4), blo = alo + (MX_TILE_BYTES >> 4);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        mx_mma(d, make_desc(alo + j * 2, DESC_B_HI), make_desc(blo + j * 2, DESC_B_HI), (j & 1) ? id1 : id0,
+                        mx_mma<PAIR>(d, make_desc(alo + j * 2, DESC_B_HI), make_desc(blo + j * 2, DESC_B_HI), (j & 1) ? id1 : id0,
                                sf + 4 * (j >> 1), sf + MT_SFB + 8 * (j >> 1), (kc > kc0 || j > 0) ? 1u : 0u);
-                    umma_commit(&bar_free[s]);
-                    if (kc == kc1 - 1) umma_commit(&bar_done[buf]);
+                    mx_commit<PAIR>(&bar_free[s]);
+                    if (kc == kc1 - 1) mx_commit<PAIR>(&bar_done[buf]);
                 }
                 __syncwarp();
-                ready = __all_sync(0xffffffffu, r_full & r_sf);
+                ready = __all_sync(0xffffffffu, r_full & r_sf & r_peer);
                 s = ns;
                 ph = nph;
             }
@@ -302,59 +364,68 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             pdl_wait();
             pdl_launch_dependents();
         }
+        // Warp w takes every fourth chunk (of fewer stages than four, as many warps as stages take turns: a barrier's parity tells
+        // only the last two rounds of a stage apart, and a warp must not look further ahead); lane l holds the scales of rows l, l + 32, ...: eight bytes of each per chunk, which lie in
+        // a scale tile as the words of one 16-byte store.  (All four warps on every chunk, a row or two a thread, took 670 cycles
+        // a chunk and were what the issuer waited for.)
+        constexpr int GROUPS = MT_MAX_N / 32;
         const int blocks = a.w.cols / 32;
         const size_t pitch = ((size_t)blocks + 15) / 16 * 16;
-        uint32_t s = 0, ph = 1;
-        bool ok = true;
+        const int step = min(4, a.stages);
+        uint32_t position = 0, s = 0, ph = 1;            // position: chunks of the units before
+        bool ok = warp < step;
         for (int u = first_unit; u < units && ok; u += unit_step) {
             Unit un;
-            if (!groups.unit(u, &un)) continue;
-            const int r0 = tid, r1 = tid + 128;
-            const bool have0 = r0 < un.n, have1 = r1 < un.n;
-            const uint4 one = make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-            const uint4* p0 = (const uint4*)(a.c.scales + (size_t)(un.row0 + (have0 ? r0 : 0)) * pitch);
-            const uint4* p1 = (const uint4*)(a.c.scales + (size_t)(un.row0 + (have1 ? r1 : 0)) * pitch);
-            uint4 n0 = one, n1 = one, c0, c1;
-            if (have0 && kc0 < kc1) n0 = p0[kc0 >> 1];
-            if (have1 && kc0 < kc1) n1 = p1[kc0 >> 1];
-            c0 = n0;
-            c1 = n1;
-            const uint32_t at0 = (r0 & 31) * 16 + (r0 >> 5) * 4;     // r1: the same in the second 512 bytes
-            for (int kc = kc0; kc < kc1 && ok; kc++) {
-                if (!(kc & 1) || kc == kc0) {
-                    c0 = n0;
-                    c1 = n1;
-                    if ((kc | 1) + 1 < kc1) {
-                        if (have0) n0 = p0[(kc >> 1) + 1];
-                        if (have1) n1 = p1[(kc >> 1) + 1];
-                    }
-                }
-                uint32_t w[4] = {(kc & 1) ? c0.z : c0.x, (kc & 1) ? c0.w : c0.y, (kc & 1) ? c1.z : c1.x, (kc & 1) ? c1.w : c1.y};
-                if (kc * 8 + 8 > blocks) {               // blocks behind the last column read as 2^0
+            if (!groups.unit_uniform(u, &un)) continue;
+            const uint8_t* base = a.c.scales + (size_t)(un.row0 + lane) * pitch;
+            uint2 next[GROUPS];
+            int kc = kc0 + (warp + step - (int)(position % step)) % step;    // this warp's first chunk of the unit
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const int left = blocks - kc * 8 - i * 4;
-                        const uint32_t keep = left >= 4 ? 0xffffffffu : left > 0 ? (1u << (8 * left)) - 1u : 0u;
-                        w[i] = (w[i] & keep) | (0x7f7f7f7fu & ~keep);
-                        w[2 + i] = (w[2 + i] & keep) | (0x7f7f7f7fu & ~keep);
+            for (int j = 0; j < GROUPS; j++)
+                if (lane + 32 * j < un.n && kc < kc1) next[j] = *(const uint2*)(base + (size_t)(32 * j) * pitch + kc * 8);
+                else next[j] = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+            s += (uint32_t)(kc - kc0);
+            while (s >= (uint32_t)a.stages) { s -= a.stages; ph ^= 1u; }
+            for (; kc < kc1 && ok; kc += step) {
+                uint32_t lo[8], hi[8];                   // blocks 0..3 and 4..7 of the lane's rows; row group 7 does not exist
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    lo[j] = j < GROUPS ? next[j < GROUPS ? j : 0].x : 0u;
+                    hi[j] = j < GROUPS ? next[j < GROUPS ? j : 0].y : 0u;
+                }
+                if (kc * 8 + 8 > blocks) {               // blocks behind the last column read as 2^0
+                    const int left = blocks - kc * 8;
+                    const uint32_t keep0 = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1u;
+                    const uint32_t keep1 = left > 4 ? (1u << (8 * (left - 4))) - 1u : 0u;
+#pragma unroll
+                    for (int j = 0; j < GROUPS; j++) {
+                        lo[j] = (lo[j] & keep0) | (0x7f7f7f7fu & ~keep0);
+                        hi[j] = (hi[j] & keep1) | (0x7f7f7f7fu & ~keep1);
                     }
                 }
-                if (lane == 0) ok = mbar_wait(&bar_free[s], ph, fail);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+#pragma unroll
+                for (int j = 0; j < GROUPS; j++)
+                    if (lane + 32 * j < un.n && kc + step < kc1) next[j] = *(const uint2*)(base + (size_t)(32 * j) * pitch + (kc + step) * 8);
+                ok = __all_sync(0xffffffffu, mbar_wait(&bar_free[s], ph, fail));
                 if (ok) {
-                    uint8_t* sfb = stage_base + s * a.stage_bytes + sfb_off;
-                    *(uint32_t*)(sfb + at0) = w[0];
-                    *(uint32_t*)(sfb + 1024 + at0) = w[1];
+                    uint4* sfb = (uint4*)(stage_base + s * a.stage_bytes + sfb_off) + lane;
+                    sfb[0] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    sfb[64] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     if (un.N > 128) {
-                        *(uint32_t*)(sfb + 512 + at0) = w[2];
-                        *(uint32_t*)(sfb + 1536 + at0) = w[3];
+                        sfb[32] = make_uint4(lo[4], lo[5], lo[6], lo[7]);
+                        sfb[96] = make_uint4(hi[4], hi[5], hi[6], hi[7]);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_sf[s]);  // always: the issuer never waits for a warp that gave up
-                if (++s == (uint32_t)a.stages) { s = 0; ph ^= 1u; }
+                s += step;
+                while (s >= (uint32_t)a.stages) { s -= a.stages; ph ^= 1u; }
             }
+            // on to the stage of the next unit's first chunk
+            position += kc1 > kc0 ? (uint32_t)(kc1 - kc0) : 0u;
+            s = position % a.stages;
+            ph = 1u ^ ((position / a.stages) & 1u);
         }
     } else {
         // ================= epilogue (TMEM lane quarter warp - 4) =================
@@ -370,7 +441,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             Unit un;
             if (!groups.unit(u, &un)) continue;
             if (kc0 >= kc1) continue;                    // this block of the cluster has no chunks
-            const int m = un.tile * 128 + q * 32 + lane;
+            const int m = (PAIR ? 2 * un.tile + rank : un.tile) * 128 + q * 32 + lane;
             const bool live = m < a.w.stored_rows;
             const uint32_t buf = done & 1u;
             ok = mbar_wait(&bar_done[buf], (done >> 1) & 1, fail);
@@ -380,7 +451,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             for (int n0 = 0; n0 < un.N; n0 += 32) {
                 uint32_t acc[32];
                 tmem_ld32(trow + buf * a.acc_cols + n0, acc);
-                if (a.split > 1) {
+                if (!PAIR && a.split > 1) {
                     // the ring is idle after a cluster's only unit: partial sums [row of the result][128] go there
                     float* part = (float*)stage_base + n0 * MX_TILE_ROWS + q * 32 + lane;
 #pragma unroll
@@ -421,12 +492,15 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_accfree[buf]);
+            if (lane == 0) {
+                if (PAIR) remote_arrive(&bar_accfree[buf], 0);       // the first block's own as well
+                else mbar_arrive(&bar_accfree[buf]);
+            }
             done++;
         }
     }
 
-    if (a.split > 1) {
+    if (!PAIR && a.split > 1) {
         // The cluster's partial sums, added in rank order; the rows of the result are dealt out to its blocks.
         const cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
@@ -468,15 +542,32 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             for (uint32_t t = produced > n ? produced - n : 0; t < produced; t++) (void)mbar_wait(&bar_full[t % n], (t / n) & 1, &none);
         }
         __syncthreads();
-        if (warp == 8 && lane == 0) {
+        if (warp == 8 && lane == 0 && (!PAIR || rank == 0)) {
             int none = 0;
-            umma_commit(&bar_drain);
+            if (PAIR)
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&bar_drain)) : "memory");
+            else umma_commit(&bar_drain);
             (void)mbar_wait(&bar_drain, 0, &none);
         }
         __syncthreads();
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (PAIR) cg::this_cluster().sync();                 // neither block leaves while the other's MMAs read its shared memory
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    if (warp == 0) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    }
+}
+
+using Kernel = void (*)(const MxTensorArgs, const CUtensorMap);
+template <bool GATED, bool PAIR> Kernel pick_kernel(int type) {
+    return type == FT_F32 ? mxfp4_tensor_kernel<FT_F32, GATED, PAIR> : type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, GATED, PAIR>
+                                                                                       : mxfp4_tensor_kernel<FT_F16, GATED, PAIR>;
+}
+Kernel pick_kernel(bool gated, int type, bool pair) {
+    return gated ? (pair ? pick_kernel<true, true>(type) : pick_kernel<true, false>(type))
+                 : (pair ? pick_kernel<false, true>(type) : pick_kernel<false, false>(type));
 }
 
 }  // namespace
@@ -529,14 +620,15 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     const int blocks = pairs ? 2 * sms : sms;
     a.stages = std::min(a.share, pairs ? half : std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes));
     if (a.split > 1) a.stages = std::max(a.stages, (a.cap * MX_TILE_ROWS * 4 + a.stage_bytes - 1) / a.stage_bytes);    // partial sums
+    int grid = a.split > 1 ? (int)units * a.split : (int)std::min<long long>(blocks, units);
+    const bool pair = !small && a.split == 1 && w.row_tiles > 1;
+    if (pair) {
+        a.stage_bytes = MX_TILE_BYTES + (a.cap / 2 + MT_BOX - 1) / MT_BOX * MT_BOX * MT_CHUNK + MT_SFB_BYTES;
+        a.stages = std::min(w.chunks, std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes));
+        grid = 2 * (int)std::min<long long>(sms / 2, passes * ((w.row_tiles + 1) / 2));
+    }
     const size_t smem = (size_t)a.stages * a.stage_bytes + 1024;
-    const int grid = a.split > 1 ? (int)units * a.split : (int)std::min<long long>(blocks, units);
-    const auto kernel = w.activation ? (c.y_type == FT_F32    ? mxfp4_tensor_kernel<FT_F32, true>
-                                        : c.y_type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, true>
-                                                              : mxfp4_tensor_kernel<FT_F16, true>)
-                                     : (c.y_type == FT_F32    ? mxfp4_tensor_kernel<FT_F32, false>
-                                        : c.y_type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, false>
-                                                              : mxfp4_tensor_kernel<FT_F16, false>);
+    const auto kernel = pick_kernel(w.activation != 0, c.y_type, pair);
     if ((e = ensure_dynamic_smem((const void*)kernel, smem)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
@@ -545,7 +637,7 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.split;
+    attr[0].val.clusterDim.x = pair ? 2 : a.split;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;

@@ -142,7 +142,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
     for (int i = 0; i < VPT; i++) {
         const int e = lane + 32 * i;
         const bool live = e < a.E && l[i] > -CUDART_INF_F;
-        if (a.bias) key[i] = live ? Q::of(score[i] + (S)__ldg(a.bias + min(e, a.E - 1))) : 0;
+        if (a.bias) key[i] = live ? Q::of(score[i] + (S)a.bias[min(e, a.E - 1)]) : 0;
         else key[i] = live ? Q::of((S)l[i]) : 0;
     }
     // Rounding errors of two keys together.  Softmax: a score is off by less than 2e-6 of the largest (its exponential by two units

@@ -175,6 +175,14 @@ def test_matmul_results(y_dtype, y_pad, activation):
         check_matmul(held, n, 203, 320, y_dtype, y_pad)
 
 
+@pytest.mark.parametrize("n,R,C,activation", [(500, 1300, 1056, None), (1000, 700, 544, "silu"), (230, 20000, 288, None), (4099, 300, 96, None),
+                                              (449, 129, 800, "gelu_tanh"), (97, 5000, 512, None), (225, 2050, 2080, "silu")])
+@pytest.mark.parametrize("y_dtype", ["f32", "bf16"])
+def test_matmul_many_rows(n, R, C, activation, y_dtype):
+    """Passes of more than 96 rows, an odd number of row tiles among them, more units than places on the chip."""
+    check_matmul(Held(n, 1, R, C, activation), n, R, C, y_dtype, seed=R)
+
+
 def test_wide_rows():
     """Rows at the documented limit, and one that leaves room for fewer tokens a pass."""
     for C in (131072, 40960):
@@ -239,6 +247,28 @@ def test_experts(name, R, C, activation):
             want, err = held.want(xv[b:t], e)
             eo.close(got[b:t], want, err, "f32", f"expert {e}")
     assert (got[live:] == 55.0).all()
+
+
+@pytest.mark.parametrize("R,C,activation", [(1300, 800, None), (650, 544, "silu"), (64, 2080, "gelu_tanh")])
+def test_experts_of_long_groups(R, C, activation):
+    """Groups around the largest pass, and a popular expert with several."""
+    import torch
+    counts = [224, 0, 225, 97, 700, 1, 448]
+    E, live = len(counts), sum(counts)
+    held = Held(R, E, R, C, activation)
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    codes, scales, xv = acts(3, live, C)
+    off, y = device(offsets), torch.full((live, R), 55.0, device="cuda")
+    torch.cuda.synchronize()
+    assert held.handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), live, y.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    got = y.double().cpu().numpy()
+    for e in range(E):
+        b, t = offsets[e], offsets[e + 1]
+        if t > b:
+            want, err = held.want(xv[b:t], e)
+            eo.close(got[b:t], want, err, "f32", f"expert {e}")
 
 
 def test_many_experts():
