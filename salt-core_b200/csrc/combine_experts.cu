@@ -25,36 +25,49 @@ struct CombineArgs {
     size_t y_stride;
 };
 
-__device__ __forceinline__ void load_picks(const CombineArgs& a, int token, long long* at, float* w) {
-    for (int j = threadIdx.x; j < a.topk; j += blockDim.x) {
-        const long long i = (long long)token * a.topk + j;
-        const long long r = a.index ? (long long)a.index[i] : i;
-        at[j] = r >= 0 && r < a.n_rows ? r : -1;
-        w[j] = a.weights[i];
+// The token's rows that exist, in their order, without gaps: the loop over them then has no branch between its loads.
+struct Picks {
+    long long at[CB_MAX_TOPK];
+    float w[CB_MAX_TOPK];
+    int n;
+};
+__device__ __forceinline__ void load_picks(const CombineArgs& a, int token, Picks& p) {
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        long long r = -1;
+        float w = 0.f;
+        if (lane < a.topk) {
+            const long long i = (long long)token * a.topk + lane;
+            r = a.index ? (long long)a.index[i] : i;
+            w = a.weights[i];
+            if (r >= a.n_rows) r = -1;
+        }
+        const uint32_t live = __ballot_sync(0xffffffffu, r >= 0);
+        const int at = __popc(live & ((1u << lane) - 1u));
+        if (r >= 0) { p.at[at] = r; p.w[at] = w; }
+        if (lane == 0) p.n = __popc(live);
     }
     __syncthreads();
 }
 
 // A block = one token and CB_THREADS pieces of eight columns.
 template <int FT> __global__ void __launch_bounds__(CB_THREADS) combine_kernel(const CombineArgs a) {
-    __shared__ long long s_at[CB_MAX_TOPK];
-    __shared__ float s_w[CB_MAX_TOPK];
+    __shared__ Picks s;
     using T = typename FloatType<FT>::T;
     const int token = blockIdx.x;
     pdl_wait();
     pdl_launch_dependents();
-    load_picks(a, token, s_at, s_w);
+    load_picks(a, token, s);
+    const int n = s.n;
     const int c = (blockIdx.y * CB_THREADS + threadIdx.x) * 8;
     if (c >= a.cols) return;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int j = 0; j < a.topk; j++) {
-        const long long r = s_at[j];
-        if (r < 0) continue;
+    for (int j = 0; j < n; j++) {
         float v[8];
-        load8<FT>((const T*)a.rows + (size_t)r * a.row_stride + c, v);
+        load8<FT>((const T*)a.rows + (size_t)s.at[j] * a.row_stride + c, v);
 #pragma unroll
-        for (int k = 0; k < 8; k++) acc[k] = __fmaf_rn(s_w[j], v[k], acc[k]);
+        for (int k = 0; k < 8; k++) acc[k] = __fmaf_rn(s.w[j], v[k], acc[k]);
     }
     const size_t o = (size_t)token * a.y_stride + c;
     if (a.y_type == FT_F32) store8<FT_F32>((float*)a.y + o, acc);
@@ -64,21 +77,19 @@ template <int FT> __global__ void __launch_bounds__(CB_THREADS) combine_kernel(c
 
 // Any column count, stride and alignment: a thread per column.
 template <int FT> __global__ void __launch_bounds__(CB_THREADS) combine_any_kernel(const CombineArgs a) {
-    __shared__ long long s_at[CB_MAX_TOPK];
-    __shared__ float s_w[CB_MAX_TOPK];
+    __shared__ Picks s;
     using T = typename FloatType<FT>::T;
     const int token = blockIdx.x;
     pdl_wait();
     pdl_launch_dependents();
-    load_picks(a, token, s_at, s_w);
+    load_picks(a, token, s);
+    const int n = s.n;
     const int c = blockIdx.y * CB_THREADS + threadIdx.x;
     if (c >= a.cols) return;
     float acc = 0.f;
 #pragma unroll 4
-    for (int j = 0; j < a.topk; j++) {
-        const long long r = s_at[j];
-        if (r >= 0) acc = __fmaf_rn(s_w[j], FloatType<FT>::up(((const T*)a.rows)[(size_t)r * a.row_stride + c]), acc);
-    }
+    for (int j = 0; j < n; j++)
+        acc = __fmaf_rn(s.w[j], FloatType<FT>::up(((const T*)a.rows)[(size_t)s.at[j] * a.row_stride + c]), acc);
     store_float(a.y, a.y_type, (size_t)token * a.y_stride + c, acc);
 }
 

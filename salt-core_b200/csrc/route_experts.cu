@@ -303,13 +303,15 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
     const bool keep = piece <= 32 * GR_HELD;
     int held[GR_HELD];
     uint32_t same[GR_HELD];
+    for (int i = tid; i < 2 * warps * a.E; i += blockDim.x) hist[i] = 0;
+    pdl_wait();                                          // the selections come from the launch before
+    pdl_launch_dependents();
 #pragma unroll
     for (int j = 0; j < GR_HELD; j++) {
         const int i = begin + 32 * j + lane;
         held[j] = i < end ? a.selected[i] : -1;
         same[j] = 0;
     }
-    for (int i = tid; i < 2 * warps * a.E; i += blockDim.x) hist[i] = 0;
     __syncthreads();
     uint32_t* mine = hist + warp * a.E;
     for (int i0 = begin; i0 < end; i0 += 32 * GR_HELD) {
@@ -367,6 +369,8 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
         base[e] = sum + before;                          // still without the experts of the threads before
         sum += all;
     }
+    // this block has read the others' totals; it leaves when all have (the wait at the end)
+    if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     uint32_t scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -426,7 +430,7 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
     }
     for (long long p = (long long)s_live + (long long)rank * blockDim.x + tid; p < a.n; p += (long long)blocks * blockDim.x)
         a.g2c[p] = -1;
-    if (cluster) cg::this_cluster().sync();              // a block's totals are read by the others until here
+    if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __host__ __device__ inline size_t group_smem(int E, int warps) { return (size_t)(2 * warps + 2) * E * sizeof(uint32_t); }
@@ -446,8 +450,6 @@ template <int VPT> __global__ void __launch_bounds__(RT_WARPS * 32) route_kernel
 __global__ void __launch_bounds__(GR_WARPS * 32) group_kernel(const GroupArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     const bool cluster = gridDim.x > 1;
-    pdl_wait();
-    pdl_launch_dependents();
     group_selections(a, (uint32_t*)smem, (int)blockIdx.x, (int)gridDim.x, cluster);
 }
 
