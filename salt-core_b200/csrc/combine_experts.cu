@@ -113,7 +113,9 @@ extern "C" int salt_b200_combine_experts(const void* d_rows, int dtype, size_t r
         return -1;
     if (tokens == 0) return 0;
     const size_t size = float_type_size(dtype), y_size = float_type_size(y_dtype);
-    if (!d_weights || !d_y || (!d_rows && n_rows > 0) || (uintptr_t)d_rows % size || (uintptr_t)d_y % y_size) return -1;
+    if (!d_weights || !d_y || (!d_rows && n_rows > 0) || (uintptr_t)d_rows % size || (uintptr_t)d_y % y_size ||
+        ((uintptr_t)d_row_index | (uintptr_t)d_weights) % 4)
+        return -1;
     CombineArgs a;
     a.rows = d_rows; a.row_stride = row_stride; a.n_rows = n_rows; a.cols = cols; a.topk = topk; a.y_type = y_dtype;
     a.index = d_row_index; a.weights = d_weights; a.y = d_y; a.y_stride = y_row_stride;

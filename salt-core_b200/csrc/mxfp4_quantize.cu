@@ -178,7 +178,7 @@ extern "C" int salt_b200_mxfp4_quantize(const void* d_x, int dtype, size_t row_s
     if (rows == 0) return 0;
     const size_t size = float_type_size(dtype);
     if ((!d_x && src_rows > 0) || !d_codes || !d_scales || (uintptr_t)d_x % 16 || row_stride * size % 16 || (uintptr_t)d_codes % 16 ||
-        (uintptr_t)d_scales % 16 || (uintptr_t)d_values % 16)
+        (uintptr_t)d_scales % 16 || (uintptr_t)d_values % 16 || (uintptr_t)d_row_index % 4)
         return -1;
     QuantArgs a;
     a.x = d_x; a.stride = row_stride; a.src_rows = src_rows; a.cols = cols; a.rows = rows; a.div = d_row_index ? index_div : 1; a.index = d_row_index;

@@ -90,7 +90,7 @@ int product(Mxfp4Weights* w, const uint8_t* codes, const uint8_t* scales, const 
             size_t y_stride, cudaStream_t stream) {
     if (!w || !on_device(w) || rows < 0 || !float_type_ok(y_type) || y_stride < (size_t)w->rows || y_stride > (size_t)1 << 40) return -1;
     if (rows == 0) return 0;
-    if (!codes || !scales || !y || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)y % float_type_size(y_type)) return -1;
+    if (!codes || !scales || !y || (uintptr_t)offsets % 4 || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)y % float_type_size(y_type)) return -1;
     Mxfp4Call c;
     c.codes = codes; c.scales = scales; c.offsets = offsets; c.rows = rows; c.y = y; c.y_type = y_type; c.y_stride = y_stride;
     return cuda_ok(launch_mxfp4_product(*w, c, stream), "mxfp4 product") ? 0 : -1;

@@ -528,7 +528,9 @@ extern "C" int salt_b200_route_experts(const SaltB200RouteSpec* spec, const void
     if (rows > 0 && (!d_logits || !d_selected || !d_weights || row_stride < (size_t)s.n_experts ||
                      (uintptr_t)d_logits % float_type_size(dtype) || (group && (!d_grouped_to_canonical || !d_canonical_to_grouped))))
         return -1;
-    if (row_stride > (size_t)1 << 40) return -1;
+    if (row_stride > (size_t)1 << 40 || ((uintptr_t)d_bias | (uintptr_t)d_selected | (uintptr_t)d_weights | (uintptr_t)d_group_offsets |
+                                         (uintptr_t)d_grouped_to_canonical | (uintptr_t)d_canonical_to_grouped) % 4)
+        return -1;
     if (rows == 0 && !group) return 0;
     RouteArgs a;
     a.logits = d_logits; a.type = dtype; a.stride = row_stride; a.rows = rows; a.E = s.n_experts; a.topk = s.topk;

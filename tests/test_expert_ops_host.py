@@ -36,6 +36,9 @@ def test_route_refuses_arguments():
     assert ex.route(s, P, 1, P, P, d_group_offsets=P, **ok) == -1        # part of a grouping
     assert ex.route(s, P, 1, P, P, d_grouped_to_canonical=P, d_canonical_to_grouped=P, **ok) == -1
     assert ex.route(s, P, 1 << 23, P, P, **ok) == -1                     # too many selections
+    for i in range(6):                                                   # misaligned tables
+        p = [P + 2 if i == j else P for j in range(6)]
+        assert ex.route(s, P, 1, *p[:5], d_bias=p[5], **ok) == -1
     assert ex._lib().salt_b200_route_experts(C.byref(s), P, 3, 64, 1, 0, P, P, 0, 0, 0, 0) == -1
     assert ex._lib().salt_b200_route_experts(None, P, 0, 64, 1, 0, P, P, 0, 0, 0, 0) == -1
     assert ex.route(s, 0, 0, 0, 0, **ok) == 0                            # no rows, no grouping: nothing to do
@@ -45,7 +48,8 @@ def test_quantize_refuses_arguments():
     ok = dict(src_rows=4, cols=64, d_codes=P, d_scales=P)
     for bad in (dict(cols=0), dict(cols=16), dict(cols=48), dict(cols=131072 + 32), dict(src_rows=-1), dict(rows=-1), dict(rows=5),
                 dict(row_stride=63), dict(row_stride=65), dict(d_codes=0), dict(d_scales=0), dict(d_codes=P + 8),
-                dict(d_scales=P + 8), dict(d_values=P + 4), dict(d_row_index=P, index_div=0)):
+                dict(d_scales=P + 8), dict(d_values=P + 4), dict(d_row_index=P, index_div=0),
+                dict(d_row_index=P + 1)):
         assert ex.quantize(P, **{**ok, **bad}) == -1, bad
     assert ex.quantize(0, **ok) == -1 and ex.quantize(P + 4, **ok) == -1
     assert ex.quantize(P, dtype="bf16", row_stride=68, **ok) == -1       # rows that begin on 8 bytes
@@ -74,7 +78,8 @@ def test_products_without_a_handle():
 def test_combine_refuses_arguments():
     ok = dict(d_rows=P, n_rows=8, cols=64, d_row_index=P, d_weights=P, tokens=2, topk=4, d_y=P)
     for bad in (dict(n_rows=-1), dict(cols=0), dict(tokens=-1), dict(topk=0), dict(topk=33), dict(d_rows=0), dict(d_weights=0),
-                dict(d_y=0), dict(row_stride=63), dict(y_row_stride=63), dict(d_rows=P + 2), dict(d_y=P + 1)):
+                dict(d_y=0), dict(row_stride=63), dict(y_row_stride=63), dict(d_rows=P + 2), dict(d_y=P + 1),
+                dict(d_row_index=P + 1), dict(d_weights=P + 2)):
         assert ex.combine(**{**ok, **bad}) == -1, bad
     assert ex.combine(**{**ok, "tokens": 0, "d_y": 0}) == 0
 

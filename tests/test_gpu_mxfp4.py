@@ -357,3 +357,109 @@ def test_repeated_and_captured(n):
     torch.cuda.synchronize()
     want, err = held.want(new[2])
     eo.close(z.double().cpu().numpy(), want, err, "f32")
+
+
+@pytest.mark.parametrize("n", [1, 40, 130, 400])
+def test_scales_far_from_one(n):
+    """Weights of 2^-107 with activations of 2^103 and the other way round: their products are near one."""
+    import torch
+    R, C = 300, 512
+    rng = np.random.default_rng(n)
+    for wb, xe in ((20, 100), (225, -104)):
+        code = rng.integers(0, 16, (1, R, C)).astype(np.uint8)
+        byte = rng.integers(wb - 2, wb + 3, (1, R, C // 32)).astype(np.uint8)
+        dev = [device(eo.mx_pack(code)), device(byte)]
+        handle = ex.Mxfp4Weights(R, C, 1, dev[0].data_ptr(), dev[1].data_ptr())
+        x = torch.randn(n, C, device="cuda") * 2.0 ** xe
+        codes, scales, _ = quantize(x, "f32")
+        xv = eo.mx_values(*eo.mx_quantize(x.double().cpu().numpy()))
+        y = torch.empty(n, R, device="cuda")
+        assert handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr()) == 0
+        want, err = eo.product(xv, eo.mx_values(code, byte)[0])
+        eo.close(y.double().cpu().numpy(), want, err, "f32", f"scales of {wb}")
+
+
+@pytest.mark.parametrize("R,activation", [(96, None), (700, "silu")])
+def test_groups_that_end_early_or_late(R, activation):
+    """No group has a row: nothing is written.  Offsets behind `rows`: rows up to there are computed, the others stay."""
+    import torch
+    E, C, n = 5, 544, 130
+    held = Held(R, E, R, C, activation)
+    codes, scales, xv = acts(9, n, C)
+    y = torch.full((n, R), 55.0, device="cuda")
+    none = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+    for rows in (1, n):
+        assert held.handle.experts(codes.data_ptr(), scales.data_ptr(), none.data_ptr(), rows, y.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0 and (y == 55.0).all()
+    off = device(np.array([0, 3, 50, 120, 125, 300], np.int32))
+    rows = 119
+    assert held.handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), rows, y.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0 and (y[rows:] == 55.0).all()
+    got = y.double().cpu().numpy()
+    for e, (b, t) in enumerate(((0, 3), (3, 50), (50, 119))):
+        want, err = held.want(xv[b:t], e)
+        eo.close(got[b:t], want, err, "f32", f"expert {e}")
+
+
+def test_two_streams_at_once():
+    """One handle used on two streams at the same time, calls of every launch form side by side."""
+    import torch
+    R, C = 1300, 1056
+    held = Held(21, 1, R, C)
+    sizes = (1, 300, 8, 90, 700, 2)
+    data = [acts(n, n, C) for n in sizes]
+    ys = [[torch.empty(n, R, device="cuda") for n in sizes] for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for k, s in enumerate(streams):
+            for i in (range(len(sizes)) if k == 0 else reversed(range(len(sizes)))):
+                assert held.handle.matmul(data[i][0].data_ptr(), data[i][1].data_ptr(), sizes[i], ys[k][i].data_ptr(), stream=s.cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    for i in range(len(sizes)):
+        assert torch.equal(ys[0][i], ys[1][i])
+        want, err = held.want(data[i][2])
+        eo.close(ys[0][i].double().cpu().numpy(), want, err, "f32", f"{sizes[i]} rows")
+
+
+def test_quantize_and_product_back_to_back():
+    """The same buffers quantised and multiplied again and again: a launch that starts early does not touch what the one before reads."""
+    import torch
+    n, R, C = 37, 700, 2080
+    held = Held(31, 1, R, C)
+    xs = [torch.randn(n, C, device="cuda") for _ in range(12)]
+    codes = torch.empty(n, C // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(n, eo.scale_pitch(C), dtype=torch.uint8, device="cuda")
+    ys = [torch.empty(n, R, device="cuda") for _ in xs]
+    torch.cuda.synchronize()
+    for x, y in zip(xs, ys):
+        assert ex.quantize(x.data_ptr(), n, C, codes.data_ptr(), scales.data_ptr()) == 0
+        assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr()) == 0
+    torch.cuda.synchronize()
+    for x, y in zip(xs, ys):
+        want, err = held.want(eo.mx_values(*eo.mx_quantize(x.double().cpu().numpy())))
+        eo.close(y.double().cpu().numpy(), want, err, "f32")
+
+
+def test_rows_beyond_32_bits():
+    """Row numbers whose byte offsets in codes and results pass 2^32: 2.2 million rows of 4096 columns, all of them zeros but a few."""
+    import torch
+    n, R, C = 2_200_003, 520, 4096
+    held = Held(41, 1, R, C)
+    codes = torch.zeros(n, C // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.full((n, eo.scale_pitch(C)), 127, dtype=torch.uint8, device="cuda")
+    at = [0, 1_048_577, 2_097_160, n - 1]
+    few = acts(3, len(at), C)
+    codes[at], scales[at] = few[0][:len(at)], few[1][:len(at)]
+    y = torch.full((n, R), 55.0, device="cuda")
+    torch.cuda.synchronize()
+    assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr()) == 0
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    want, err = held.want(few[2])
+    eo.close(y[at].double().cpu().numpy(), want, err, "f32")
+    y[at] = 0
+    assert not y.any()

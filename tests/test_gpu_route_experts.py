@@ -113,6 +113,28 @@ def test_equal_logits_and_masks(scoring, biased, groups):
         check(rows.cuda(), 6, bias=bias, scoring=scoring, n_groups=groups, topk_groups=min(groups, 2), group_top=2, renormalize=renorm)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_bias_that_is_not_a_number(scoring, groups):
+    """A bias of NaN or -infinity takes an expert out, +infinity puts it first; neither enters a weight."""
+    bias = np.linspace(-0.2, 0.2, 64)
+    bias[[3, 20]], bias[[7, 40]], bias[[12, 55]] = np.nan, -np.inf, np.inf
+    check(logits_of(8, 70, 64, "f32"), 5, bias=bias, scoring=scoring, n_groups=groups, topk_groups=min(groups, 3), group_top=1)
+
+
+def test_more_selections_than_registers_hold():
+    """65536 selections and more: a warp's piece is longer than what it keeps between its two passes; all for one expert, too."""
+    import torch
+    for T, E, topk, spread in ((9001, 64, 8, 2.0), (70000, 16, 1, 2.0), (70000, 600, 1, 2.0), (70000, 8, 1, 0.0)):
+        l = logits_of(T, T, E, "f32", spread)
+        sel, w, off, g2c, c2g = run(l, topk)
+        order = torch.sort(torch.from_numpy(sel.reshape(-1).astype(np.int64)), stable=True).indices.numpy()
+        assert np.array_equal(g2c, order) and np.array_equal(c2g[g2c], np.arange(T * topk))
+        assert np.array_equal(off, np.concatenate(([0], np.cumsum(np.bincount(sel.reshape(-1), minlength=E)))))
+        want = torch.sort(l.double(), dim=1, descending=True, stable=True).indices[:, :topk].sort(dim=1).values
+        assert np.array_equal(sel, want.cpu().numpy())
+
+
 def test_scores_too_small_for_32_bits():
     import torch
     l = torch.full((3, 64), -300.0, device="cuda") - torch.arange(64, device="cuda")[None]
