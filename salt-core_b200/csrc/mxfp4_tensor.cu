@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/salt_gpu_b200.h"
 #include "float_types.cuh"
@@ -39,7 +40,7 @@ constexpr uint32_t MT_SF_STRIDE = 32, MT_SFB = 8;
 constexpr int MT_SFB_BYTES = 2048;
 constexpr int MT_MAX_STAGES = 8;
 constexpr int MT_MAX_SPLIT = 8;
-constexpr int MT_SMEM = 220 * 1024, MT_SMALL_SMEM = 103 * 1024;
+constexpr int MT_SMEM = 217 * 1024, MT_SMALL_SMEM = 103 * 1024;
 
 struct MxTensorArgs {
     Mxfp4Weights w;
@@ -47,6 +48,7 @@ struct MxTensorArgs {
     int cap;                             // most rows of a pass, a multiple of 16
     int stages, stage_bytes;
     uint32_t tmem_cols, acc_cols;        // columns of TMEM, and of one of the two accumulators at its start
+    int staged;                          // results go through shared memory behind the ring (long passes, rows that begin on 16 bytes)
     int split, share;                    // blocks of a cluster that share a unit, and most of its chunks that one takes
 };
 
@@ -113,7 +115,7 @@ __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, 
 struct Unit { int expert, tile, row0, n, N; };   // n rows of the pass, N = n up to a multiple of 16
 
 // Passes of a group of n rows: as few as the cap allows, of equal size up to the multiple of 16.
-__device__ __forceinline__ int pass_rows(int n, int cap) {
+__host__ __device__ __forceinline__ int pass_rows(int n, int cap) {
     const int passes = (n + cap - 1) / cap;
     return passes ? ((n + passes - 1) / passes + 15) & ~15 : cap;
 }
@@ -429,6 +431,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         }
     } else {
         // ================= epilogue (TMEM lane quarter warp - 4) =================
+        constexpr int WIDTH = MX_TILE_ROWS / (GATED ? 2 : 1);        // results of a tile per row
         const int q = warp - 4;
         const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16);
         uint32_t done = 0;
@@ -443,6 +446,9 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             if (kc0 >= kc1) continue;                    // this block of the cluster has no chunks
             const int m = (PAIR ? 2 * un.tile + rank : un.tile) * 128 + q * 32 + lane;
             const bool live = m < a.w.stored_rows;
+            // A store per row of the result writes 64 bytes a warp and takes some nine cycles of the SM; 16 bytes a lane, of rows that
+            // lie together in shared memory, are four times less of them.
+            const bool stage_out = a.staged && m - q * 32 - lane + MX_TILE_ROWS <= a.w.stored_rows;
             const uint32_t buf = done & 1u;
             ok = mbar_wait(&bar_done[buf], (done >> 1) & 1, fail);
             ok = __all_sync(0xffffffffu, ok);
@@ -457,36 +463,48 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
 #pragma unroll
                     for (int k = 0; k < 32; k++)
                         if (n0 + k < un.N) part[k * MX_TILE_ROWS] = __uint_as_float(acc[k]);
-                } else if (GATED) {
-                    // lanes 2 i and 2 i + 1 hold gate and up of the same result: the even lane takes even rows, the odd lane odd ones
-                    const bool odd = lane & 1;
-                    T* y = (T*)a.c.y + (size_t)(un.row0 + n0 + odd) * a.c.y_stride + (m >> 1);
-                    const int left = live ? un.n - n0 - odd : 0;     // rows k = 0, 2, ... below it exist
-                    float v[16];
-#pragma unroll
-                    for (int k = 0; k < 16; k++) {
-                        const float mine = __uint_as_float(odd ? acc[2 * k + 1] : acc[2 * k]);
-                        const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? acc[2 * k] : acc[2 * k + 1]), 1);
-                        v[k] = gate_act(a.w.activation, odd ? other : mine) * (odd ? mine : other);
-                    }
-                    if (left >= 31) {                    // all 32 rows: no branch between the activations
-#pragma unroll
-                        for (int k = 0; k < 16; k++) y[(size_t)(2 * k) * a.c.y_stride] = FloatType<FT>::down(v[k]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 16; k++)
-                            if (2 * k < left) y[(size_t)(2 * k) * a.c.y_stride] = FloatType<FT>::down(v[k]);
-                    }
                 } else {
-                    T* y = (T*)a.c.y + (size_t)(un.row0 + n0) * a.c.y_stride + m;
-                    const int left = live ? un.n - n0 : 0;
-                    if (left >= 32) {
+                    T out[32];                           // of a gated pair 16
+                    const bool odd = lane & 1;
+                    if (GATED) {
+                        // lanes 2 i and 2 i + 1 hold gate and up of the same result: the even lane takes even rows, the odd lane odd ones
 #pragma unroll
-                        for (int k = 0; k < 32; k++) y[(size_t)k * a.c.y_stride] = FloatType<FT>::down(__uint_as_float(acc[k]));
+                        for (int k = 0; k < 16; k++) {
+                            const float mine = __uint_as_float(odd ? acc[2 * k + 1] : acc[2 * k]);
+                            const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(odd ? acc[2 * k] : acc[2 * k + 1]), 1);
+                            out[k] = FloatType<FT>::down(gate_act(a.w.activation, odd ? other : mine) * (odd ? mine : other));
+                        }
                     } else {
 #pragma unroll
-                        for (int k = 0; k < 32; k++)
-                            if (k < left) y[(size_t)k * a.c.y_stride] = FloatType<FT>::down(__uint_as_float(acc[k]));
+                        for (int k = 0; k < 32; k++) out[k] = FloatType<FT>::down(__uint_as_float(acc[k]));
+                    }
+                    if (stage_out) {
+                        T* slab = (T*)(stage_base + a.stages * a.stage_bytes);
+                        asm volatile("bar.sync 1, 128;" ::: "memory");   // the slab before this one has been stored
+#pragma unroll
+                        for (int k = 0; k < (GATED ? 16 : 32); k++)
+                            if (GATED) slab[(2 * k + odd) * WIDTH + (q * 32 + lane) / 2] = out[k];
+                            else slab[k * WIDTH + q * 32 + lane] = out[k];
+                        asm volatile("bar.sync 1, 128;" ::: "memory");
+                        constexpr int PIECES = WIDTH * (int)sizeof(T) / 16;
+                        T* y = (T*)a.c.y + (size_t)(un.row0 + n0) * a.c.y_stride + (m - q * 32 - lane) / (GATED ? 2 : 1);
+                        const int pieces = min(32, un.n - n0) * PIECES;
+                        for (int i = q * 32 + lane; i < pieces; i += 128) {
+                            const int r = i / PIECES, c = i % PIECES;
+                            ((uint4*)(y + (size_t)r * a.c.y_stride))[c] = ((const uint4*)(slab + r * WIDTH))[c];
+                        }
+                    } else {
+                        T* y = (T*)a.c.y + (size_t)(un.row0 + n0 + (GATED && odd)) * a.c.y_stride + (GATED ? m >> 1 : m);
+                        const int left = live ? un.n - n0 - (GATED && odd) : 0;      // rows below it exist
+                        constexpr int STEP = GATED ? 2 : 1;
+                        if (left > 32 - STEP) {          // all of them: no branch between the stores
+#pragma unroll
+                            for (int k = 0; k < 32 / STEP; k++) y[(size_t)(STEP * k) * a.c.y_stride] = out[k];
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 32 / STEP; k++)
+                                if (STEP * k < left) y[(size_t)(STEP * k) * a.c.y_stride] = out[k];
+                        }
                     }
                 }
             }
@@ -560,6 +578,34 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
     }
 }
 
+// Most rows of a pass, for `groups` groups that are expected to have `rows` rows (of expert groups a quarter and 8 above the average:
+// a longer one takes a pass more, which reads its weights again, from L2).  Longer passes load less in all; shorter ones keep more
+// SMs busy, write their results sooner, and up to 96 rows two blocks share an SM.  Microseconds by what was measured: a chunk takes a
+// block 0.3, or 0.4 with a second one beside it, a column of results 0.022, and all SMs together load 11 TB/s from L2.  64
+// experts of 1536 x 5120, 16 / 31 / 63 rows on average: 58 / 89 / 93 us by passes of up to 96, 65 / 99 / 104 by longer ones; 125
+// rows: 130 and 111.
+int choose_cap(int rows, int groups, int row_tiles, int chunks, int sms) {
+    int best = 0;
+    double least = 0, fewest = 0;
+    for (int cap = MT_BOX; cap <= MT_MAX_N; cap += MT_BOX) {
+        const double passes = (double)groups * ((rows + cap - 1) / cap), units = passes * row_tiles;
+        const int n = pass_rows(rows, cap);
+        const bool two = cap <= MT_SMALL_N && units > sms;
+        const double rounds = std::ceil(units / (two ? 2 * sms : sms)), loop = chunks * (two ? 0.4 : 0.3), store = 0.022 * n;
+        const double loads = units * chunks * (MX_TILE_BYTES + (cap > MT_SMALL_N ? n / 2 : n) * MT_CHUNK) / 11e6;
+        const double t = std::max(rounds * std::max(loop, store) + std::min(loop, store), loads);
+        // as many passes by more room for them: no gain; a tenth is within what the estimate leaves out (37 rows of 2112 x 2816: 6.4 us
+        // in one pass, 7.1 in two)
+        if (!best || (passes < fewest && t < 1.1 * least)) {
+            best = cap;
+            least = t;
+            fewest = passes;
+        }
+        if (cap >= rows) break;
+    }
+    return best;
+}
+
 using Kernel = void (*)(const MxTensorArgs, const CUtensorMap);
 template <bool GATED, bool PAIR> Kernel pick_kernel(int type) {
     return type == FT_F32 ? mxfp4_tensor_kernel<FT_F32, GATED, PAIR> : type == FT_BF16 ? mxfp4_tensor_kernel<FT_BF16, GATED, PAIR>
@@ -586,12 +632,9 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     MxTensorArgs a;
     a.w = w;
     a.c = c;
-    // Rows of a pass.  A dense product takes what it has.  Groups: a quarter and 16 above the average; a longer group takes a pass
-    // more, which reads its weights again from L2.  Passes of up to 96 rows leave room for two blocks per SM (64 experts of
-    // 1536 x 5120, 16 / 31 / 63 rows on average: 58 / 89 / 93 us against 65 / 99 / 104 with one; at 125, in two passes each, 130
-    // against 111).
-    const int expect = c.offsets ? std::min(c.rows, (int)(1.25 * c.rows / w.experts) + 16) : c.rows;
-    a.cap = std::min(MT_MAX_N, (expect + MT_BOX - 1) / MT_BOX * MT_BOX);
+    const int sms = device_sms();
+    a.cap = choose_cap(c.offsets ? (int)(1.25 * c.rows / w.experts) + 8 : c.rows, c.offsets ? std::min(c.rows, w.experts) : 1, w.row_tiles,
+                       w.chunks, sms);
     a.stage_bytes = MX_TILE_BYTES + a.cap * MT_CHUNK + MT_SFB_BYTES;
     const bool small = a.cap <= MT_SMALL_N;
     a.acc_cols = small ? MT_SMALL_N : MT_MAX_N;
@@ -602,7 +645,7 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     // 4096 x 4096, one row: 8.3 / 6.9 / 6.8 us by clusters of 1 / 2 / 4; 5120 x 1536, 32 rows: 4.8 / 6.4.  Blocks that wait for a
     // place cost more than they save: 96 units of 20 chunks 13.1 / 13.8 / 19.6.  Clusters of blocks that fill an SM each do not
     // cover all SMs (17 of eight blocks: 11.9 us against 6.2 for 17 of four).
-    const int sms = device_sms(), places = small ? sms + sms / 12 : sms - sms / 8;
+    const int places = small ? sms + sms / 12 : sms - sms / 8;
     a.split = 1;
     a.share = w.chunks;
     int cost = w.chunks;
@@ -622,12 +665,15 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     if (a.split > 1) a.stages = std::max(a.stages, (a.cap * MX_TILE_ROWS * 4 + a.stage_bytes - 1) / a.stage_bytes);    // partial sums
     int grid = a.split > 1 ? (int)units * a.split : (int)std::min<long long>(blocks, units);
     const bool pair = !small && a.split == 1 && w.row_tiles > 1;
+    const size_t y_size = float_type_size(c.y_type);
+    a.staged = !small && a.split == 1 && (uintptr_t)c.y % 16 == 0 && c.y_stride * y_size % 16 == 0;
+    const int slab = a.staged ? MT_BOX * MX_TILE_ROWS / (w.activation ? 2 : 1) * (int)y_size : 0;
     if (pair) {
         a.stage_bytes = MX_TILE_BYTES + (a.cap / 2 + MT_BOX - 1) / MT_BOX * MT_BOX * MT_CHUNK + MT_SFB_BYTES;
-        a.stages = std::min(w.chunks, std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes));
         grid = 2 * (int)std::min<long long>(sms / 2, passes * ((w.row_tiles + 1) / 2));
     }
-    const size_t smem = (size_t)a.stages * a.stage_bytes + 1024;
+    if (!small && a.split == 1) a.stages = std::min(w.chunks, std::min(MT_MAX_STAGES, (MT_SMEM - 1024 - slab) / a.stage_bytes));
+    const size_t smem = (size_t)a.stages * a.stage_bytes + slab + 1024;
     const auto kernel = pick_kernel(w.activation != 0, c.y_type, pair);
     if ((e = ensure_dynamic_smem((const void*)kernel, smem)) != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
