@@ -198,10 +198,11 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
             if (g == at) mine = 0;
         }
         if (!decided) return false;
+        const uint32_t inverse = ((1u << 20) + per - 1) / per;       // e / per for e * per below 2^20
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
             const int e = lane + 32 * i;
-            if (e < a.E && !((stay >> (e / per)) & 1u)) key[i] = 0;
+            if (e < a.E && !((stay >> (((uint32_t)e * inverse) >> 20)) & 1u)) key[i] = 0;
         }
     }
     uint32_t taken = 0;                                  // bit i: expert lane + 32 i is selected
