@@ -1,5 +1,6 @@
 // The experts' rows of every token back in token order: y[t] = sum_j w[t][j] * rows[index[t][j]], j ascending, in 32 bits and
-// rounded once.  One read of every row that is used and one write per token: bound by memory.
+// rounded once.  One read of every row that is used and one write per token: bound by memory (1999 tokens of four rows of 5120
+// bf16: 18.8 us, 5.4 TB/s).
 #include <algorithm>
 
 #include "../../include/salt_gpu_b200.h"

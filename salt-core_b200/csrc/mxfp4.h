@@ -6,8 +6,8 @@
 namespace sb {
 
 // Layout made once at creation: per 128 stored rows and 256 columns one tile of 17 KB that a single bulk copy brings into shared
-// memory as the tensor core reads it, tiles of a row block next to one another.  (Rows of codes side by side, as they come, cost
-// 128 separate lines of 128 bytes per tile: 535 MB of experts then streamed at 3.7 TB/s.)
+// memory as the tensor core reads it, tiles of a row block next to one another.  (Rows of codes side by side, as they come, are 128 separate lines
+// of 128 bytes per tile and two kinds of copies.)
 //   16384 bytes of codes: row r at r * 128, its 16-byte piece c (one block of 32 columns) at place c ^ (r % 8);
 //   1024 bytes of scales: block c of row r at (c / 4) * 512 + (r % 32) * 16 + (r / 32) * 4 + c % 4.
 // A gated pair is stored with its rows alternating (gate row i at 2 i, up row i at 2 i + 1), so that the two values an activation

@@ -2,10 +2,18 @@
 // columns of each, 32-bit accumulation in TMEM), dense or by expert groups.
 //
 // A unit = 128 stored weight rows (M) times one pass of a group's rows (N, a multiple of 16), K in chunks of 256 columns = one
-// 128-byte row of packed codes = four MMAs of K = 64.  Persistent blocks, one per SM; unit u of the launch goes to block u mod
-// grid, a group's row tiles next to one another, so the blocks that work at the same time read the same activations.  Which
-// group a unit belongs to is found in a prefix table over the groups' passes, made by every block from the device offsets.
-// Where the units are few, a cluster of 2 to 8 blocks shares each, K split; the partial sums meet in distributed shared memory.
+// 128-byte row of packed codes = four MMAs of K = 64.  Persistent blocks; unit u of the launch goes to block u mod grid, a
+// group's row tiles next to one another, so the blocks that work at the same time read the same activations.  Which group a
+// unit belongs to is found in a prefix table over the groups' passes, made by every block from the device offsets.
+// Four launch forms, by a rule at the launch:
+//   passes of up to 96 rows: two blocks per SM, half of TMEM each; what bounds them is HBM (64 experts of 1536 x 5120, gate | up, 16 /
+//     31 / 63 rows each: 58 / 89 / 93 us, the last two 6.0 TB/s of 6.5 measured);
+//   few units: a cluster of 2 to 8 blocks shares each, K split, and the partial sums meet in distributed shared memory; latency (one
+//     row of 4096 x 4096: 7.2 us);
+//   longer passes: a pair of SMs (cta_group::2) takes two row tiles of a pass and each loads half of its rows.  Loads from L2
+//     bounded one SM per unit (11 TB/s in all: 4096 x 5120 x 5120 55 us, 46.7 in pairs); now the tensor pipe is busy 60 % of the
+//     cycles, the rest is the scale copies before each chunk's MMAs, six rounds of units where 5.1 would do, first loads and last stores;
+//   the same with one SM per unit, where there is a single row tile.
 // Warp roles:
 //   warp 9      producer: one bulk copy of the weight tile, codes and scales, which lies in memory as the tensor core reads it, and
 //               TMA copies of the rows' codes (boxes of 32 rows, 128-byte swizzle)
@@ -331,7 +339,8 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
                 if (!ready) ok = __all_sync(0xffffffffu, mbar_wait2(&bar_full[s], ph, &bar_sf[s], ph, fail));
                 if (PAIR && !ready && ok) ok = __all_sync(0xffffffffu, mbar_wait(&bar_peer[s], ph, fail));
                 if (!ok) break;
-                // the next stage's barriers are asked before this stage's MMAs go out: an answer takes some 130 cycles
+                // The next stage's barriers are asked before this stage's MMAs go out: an answer takes some 130 cycles.  (Asking two
+                // stages ahead, to copy the next chunk's scales before this chunk's MMAs, cost more than it hid: 46.7 -> 49.8 us.)
                 const uint32_t ns = s + 1 == (uint32_t)a.stages ? 0 : s + 1, nph = ns ? ph : ph ^ 1u;
                 const uint32_t r_full = mbar_test(&bar_full[ns], nph), r_sf = mbar_test(&bar_sf[ns], nph), r_peer = PAIR ? mbar_test(&bar_peer[ns], nph) : 1u;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -367,8 +376,8 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             pdl_launch_dependents();
         }
         // Warp w takes every fourth chunk (of fewer stages than four, as many warps as stages take turns: a barrier's parity tells
-        // only the last two rounds of a stage apart, and a warp must not look further ahead); lane l holds the scales of rows l, l + 32, ...: eight bytes of each per chunk, which lie in
-        // a scale tile as the words of one 16-byte store.  (All four warps on every chunk, a row or two a thread, took 670 cycles
+        // only the last two rounds of a stage apart, and a warp must not look further ahead); lane l holds the scales of rows l,
+        // l + 32, ...: eight bytes of each per chunk, which lie in a scale tile as the words of one 16-byte store.  (All four warps on every chunk, a row or two a thread, took 670 cycles
         // a chunk and were what the issuer waited for.)
         constexpr int GROUPS = MT_MAX_N / 32;
         const int blocks = a.w.cols / 32;
