@@ -651,7 +651,7 @@ typedef struct SaltB200Mxfp4Spec {
 int salt_b200_mxfp4_weights_create(const SaltB200Mxfp4Spec *spec, void *stream, void **weights_out);
 int salt_b200_mxfp4_weights_destroy(void *weights);      /* after every call that uses it has finished */
 /* y[i] = W x_i for `rows` quantised rows; n_experts must be 1.  d_y [rows][y_row_stride] of y_dtype.  Sums in 32 bits, rounded once.
- * A block's scale product and sum must lie within the range of 32 bits. */
+ * rows is at most 2^30. A block's scale product and sum must lie within the range of 32 bits. */
 int salt_b200_mxfp4_matmul(void *weights, const uint8_t *d_codes, const uint8_t *d_scales, int rows, void *d_y, int y_dtype,
                            size_t y_row_stride, void *stream);
 /* The same with row i multiplied by the matrix of its group: rows d_group_offsets[e] .. d_group_offsets[e + 1] (ascending) are

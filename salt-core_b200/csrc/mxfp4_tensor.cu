@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
                             const int r = i / PIECES, c = i % PIECES;
                             ((uint4*)(y + (size_t)r * a.c.y_stride))[c] = ((const uint4*)(slab + r * WIDTH))[c];
                         }
+                        __syncwarp();
                     } else {
                         T* y = (T*)a.c.y + (size_t)(un.row0 + n0 + (GATED && odd)) * a.c.y_stride + (GATED ? m >> 1 : m);
                         const int left = live ? un.n - n0 - (GATED && odd) : 0;      // rows below it exist
@@ -642,7 +643,7 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     a.w = w;
     a.c = c;
     const int sms = device_sms();
-    a.cap = choose_cap(c.offsets ? (int)(1.25 * c.rows / w.experts) + 8 : c.rows, c.offsets ? std::min(c.rows, w.experts) : 1, w.row_tiles,
+    a.cap = choose_cap(c.offsets ? (int)std::min(1.25 * c.rows / w.experts + 8, 1e9) : c.rows, c.offsets ? std::min(c.rows, w.experts) : 1, w.row_tiles,
                        w.chunks, sms);
     a.stage_bytes = MX_TILE_BYTES + a.cap * MT_CHUNK + MT_SFB_BYTES;
     const bool small = a.cap <= MT_SMALL_N;
@@ -650,24 +651,24 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     a.tmem_cols = small ? 256 : 512;
     const long long passes = c.offsets ? std::min<long long>(c.rows, c.rows / a.cap + w.experts) : (c.rows + a.cap - 1) / a.cap;
     const long long units = passes * w.row_tiles;
+    if (units > INT32_MAX / 2) return cudaErrorInvalidValue;
     // Few units: a cluster shares each.  Joining the parts costs about as much as four to six chunks of one block (0.33 us each):
     // 4096 x 4096, one row: 8.3 / 6.9 / 6.8 us by clusters of 1 / 2 / 4; 5120 x 1536, 32 rows: 4.8 / 6.4.  Blocks that wait for a
     // place cost more than they save: 96 units of 20 chunks 13.1 / 13.8 / 19.6.  Clusters of blocks that fill an SM each do not
     // cover all SMs (17 of eight blocks: 11.9 us against 6.2 for 17 of four).
-    const int places = small ? sms + sms / 12 : sms - sms / 8;
+    const int half = std::min(MT_MAX_STAGES, (MT_SMALL_SMEM - 1024) / a.stage_bytes);
     a.split = 1;
     a.share = w.chunks;
     int cost = w.chunks;
-    for (int split = 2; split <= MT_MAX_SPLIT && units * split <= places; split *= 2) {
-        const int share = (w.chunks + split - 1) / split;
-        if (share + 4 + split / 4 < cost) {
+    for (int split = 2; split <= MT_MAX_SPLIT; split *= 2) {
+        const int share = (w.chunks + split - 1) / split, places = small && share <= half ? sms + sms / 12 : sms - sms / 8;
+        if (units * split <= places && share + 4 + split / 4 < cost) {
             a.split = split;
             a.share = share;
             cost = share + 4 + split / 4;
         }
     }
     // Two blocks per SM where there is work for them or where half the stages hold all chunks; otherwise one with twice the stages
-    const int half = std::min(MT_MAX_STAGES, (MT_SMALL_SMEM - 1024) / a.stage_bytes);
     const bool pairs = small && (units * a.split > sms || a.share <= half);
     const int blocks = pairs ? 2 * sms : sms;
     a.stages = std::min(a.share, pairs ? half : std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes));

@@ -88,7 +88,7 @@ bool upload(const SaltB200Mxfp4Spec& s, Mxfp4Weights* w, uint8_t* staged, cudaSt
 
 int product(Mxfp4Weights* w, const uint8_t* codes, const uint8_t* scales, const int32_t* offsets, int rows, void* y, int y_type,
             size_t y_stride, cudaStream_t stream) {
-    if (!w || !on_device(w) || rows < 0 || !float_type_ok(y_type) || y_stride < (size_t)w->rows || y_stride > (size_t)1 << 40) return -1;
+    if (!w || !on_device(w) || rows < 0 || rows > 1 << 30 || !float_type_ok(y_type) || y_stride < (size_t)w->rows || y_stride > (size_t)1 << 40) return -1;
     if (rows == 0) return 0;
     if (!codes || !scales || !y || (uintptr_t)offsets % 4 || (uintptr_t)codes % 16 || (uintptr_t)scales % 16 || (uintptr_t)y % float_type_size(y_type)) return -1;
     Mxfp4Call c;

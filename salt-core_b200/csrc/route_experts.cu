@@ -39,6 +39,7 @@ constexpr int GR_WARPS = 32;
 constexpr int GR_HELD = 8;               // selections of a lane that stay in registers between the two passes
 constexpr int GR_CLUSTER = 8;
 constexpr int GR_FEW = 512;              // RT_FUSED_TOKENS times the largest top-k
+constexpr size_t GR_MAX_SMEM = 200 * 1024;
 constexpr int GR_ONE_BLOCK = 2048;       // selections that one block groups by itself
 constexpr unsigned FULL = 0xffffffffu;
 
@@ -57,6 +58,7 @@ struct GroupArgs {
     const int32_t* selected;
     int n, E;
     int32_t *offsets, *g2c, *c2g;
+    int ordered;                         // a block's selections fit into shared memory in the order of their groups
 };
 
 // Bit patterns that order like the values, -0 like +0; 0 is below every finite one and stands for "none".
@@ -294,16 +296,20 @@ __device__ __forceinline__ uint32_t same_expert(uint32_t* bits, int e, bool ok, 
 }
 
 __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, int blocks, bool cluster) {
-    __shared__ uint32_t s_part[32], s_live;
+    using Sums = unsigned long long;                     // low word: of the whole grouping, high word: of this block's part
+    __shared__ Sums s_part[32], s_live;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
     uint32_t* bits = hist + (warps + warp) * a.E;        // this warp's words
     uint32_t* total = hist + 2 * warps * a.E;            // this block's selections of every expert
     uint32_t* base = total + a.E;                        // where this block's part of the group begins
+    uint32_t* local = base + a.E;                        // where it begins among the block's selections
+    uint32_t* order = local + a.E;                       // the block's selections in that order: expert << 16 | number in the block
     const int piece = ((a.n + warps * blocks - 1) / (warps * blocks) + 31) & ~31;
     const int w_all = rank * warps + warp;
     const int begin = (int)min((long long)w_all * piece, (long long)a.n);
     const int end = (int)min((long long)begin + piece, (long long)a.n);
     const bool keep = piece <= 32 * GR_HELD;
+    const int block_begin = rank * warps * piece;        // read only where the pieces are short
     int held[GR_HELD];
     uint32_t same[GR_HELD];
     for (int i = tid; i < 2 * warps * a.E; i += blockDim.x) hist[i] = 0;
@@ -354,7 +360,7 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
     else __syncthreads();
     // offsets of the groups: a thread sums a run of experts, then the threads' sums are scanned
     const int run = (a.E + (int)blockDim.x - 1) / (int)blockDim.x;
-    uint32_t sum = 0;
+    Sums sum = 0;
     for (int j = 0; j < run; j++) {
         const int e = tid * run + j;
         if (e >= a.E) break;
@@ -369,40 +375,43 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
         } else {
             all = total[e];
         }
-        base[e] = sum + before;                          // still without the experts of the threads before
-        sum += all;
+        base[e] = (uint32_t)sum + before;                // still without the experts of the threads before
+        local[e] = (uint32_t)(sum >> 32);
+        sum += (Sums)total[e] << 32 | all;
     }
     // this block has read the others' totals; it leaves when all have (the wait at the end)
-    if (cluster) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    uint32_t scan = sum;
+    if (cluster) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    Sums scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t o = __shfl_up_sync(FULL, scan, d);
+        const Sums o = __shfl_up_sync(FULL, scan, d);
         if (lane >= d) scan += o;
     }
     if (lane == 31) s_part[warp] = scan;
     __syncthreads();
     if (warp == 0) {
-        uint32_t p = lane < warps ? s_part[lane] : 0;
+        Sums p = lane < warps ? s_part[lane] : 0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t o = __shfl_up_sync(FULL, p, d);
+            const Sums o = __shfl_up_sync(FULL, p, d);
             if (lane >= d) p += o;
         }
         if (lane < warps) s_part[lane] = p;
         if (lane == 31) s_live = p;
     }
     __syncthreads();
-    const uint32_t front = scan - sum + (warp ? s_part[warp - 1] : 0u);
+    const Sums front = scan - sum + (warp ? s_part[warp - 1] : 0ull);
     for (int j = 0; j < run; j++) {
         const int e = tid * run + j;
         if (e >= a.E) break;
-        base[e] += front;
+        base[e] += (uint32_t)front;
+        local[e] += (uint32_t)(front >> 32);
     }
     __syncthreads();
+    const uint32_t live = (uint32_t)s_live;
     if (rank == 0) {                                     // block 0: nothing before its part, so base is the offset
         for (int e = tid; e < a.E; e += blockDim.x) a.offsets[e] = (int32_t)base[e];
-        if (tid == 0) a.offsets[a.E] = (int32_t)s_live;
+        if (tid == 0) a.offsets[a.E] = (int32_t)live;
     }
     for (int i0 = begin; i0 < end; i0 += 32 * GR_HELD) {
         if (!keep) {
@@ -419,11 +428,12 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
             const bool ok = e >= 0 && e < a.E;
             const uint32_t lanes = keep ? same[j] : same_expert(bits, e, ok, lane);
             uint32_t p = 0;
-            if (ok) p = base[e] + mine[e] + __popc(lanes & ((1u << lane) - 1u));
+            if (ok) p = mine[e] + __popc(lanes & ((1u << lane) - 1u));       // among the block's selections of this expert
             __syncwarp();
             if (ok) {
-                a.g2c[p] = i;
-                a.c2g[i] = (int32_t)p;
+                if (a.ordered) order[local[e] + p] = (uint32_t)e << 16 | (uint32_t)(i - block_begin);
+                else a.g2c[base[e] + p] = i;
+                a.c2g[i] = (int32_t)(base[e] + p);
                 if (lane == __ffs(lanes) - 1) mine[e] += __popc(lanes);
             } else if (i < end) {
                 a.c2g[i] = -1;
@@ -431,12 +441,20 @@ __device__ void group_selections(const GroupArgs& a, uint32_t* hist, int rank, i
             __syncwarp();
         }
     }
-    for (long long p = (long long)s_live + (long long)rank * blockDim.x + tid; p < a.n; p += (long long)blocks * blockDim.x)
+    if (a.ordered) {                                     // out group by group: runs of neighbours instead of single words
+        __syncthreads();
+        const uint32_t mine_all = (uint32_t)(s_live >> 32);
+        for (uint32_t p = tid; p < mine_all; p += blockDim.x) {
+            const uint32_t v = order[p], e = v >> 16;
+            a.g2c[base[e] + p - local[e]] = block_begin + (int)(v & 0xffffu);
+        }
+    }
+    for (long long p = (long long)live + (long long)rank * blockDim.x + tid; p < a.n; p += (long long)blocks * blockDim.x)
         a.g2c[p] = -1;
-    if (cluster) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (cluster) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-__host__ __device__ inline size_t group_smem(int E, int warps) { return (size_t)(2 * warps + 2) * E * sizeof(uint32_t); }
+__host__ __device__ inline size_t group_smem(int E, int warps) { return (size_t)(2 * warps + 3) * E * sizeof(uint32_t); }
 __host__ __device__ inline size_t route_smem(int E, int groups, int warps) {
     return groups > 1 ? (size_t)warps * E * sizeof(unsigned long long) : 0;
 }
@@ -505,10 +523,16 @@ template <int VPT> cudaError_t launch_route(const RouteArgs& a, const GroupArgs*
     }
     if (!g) return cudaSuccess;
     const int warps = a.E <= 512 ? GR_WARPS : GR_WARPS / 2;          // two words per expert and warp: at most 139 KB
-    const size_t smem = group_smem(a.E, warps);
+    GroupArgs ga = *g;
+    const int blocks = ga.n > GR_ONE_BLOCK ? GR_CLUSTER : 1;
+    const long long held = (ga.n + (long long)warps * blocks - 1) / (warps * blocks);      // of a warp
+    const long long part = (held + 31) / 32 * 32 * warps;           // of a block
+    size_t smem = group_smem(a.E, warps);
+    ga.ordered = part <= 0xffff && smem + part * 4 <= GR_MAX_SMEM;
+    if (ga.ordered) smem += part * 4;
     if (smem > PLAIN_DYNAMIC_SMEM && (e = ensure_dynamic_smem((const void*)group_kernel, smem)) != cudaSuccess) return e;
-    if (g->n > GR_ONE_BLOCK) return launch_pdl_cluster(group_kernel, GR_CLUSTER, dim3(warps * 32), smem, stream, *g);
-    return launch_pdl(group_kernel, dim3(1), dim3(warps * 32), smem, stream, *g);
+    if (blocks > 1) return launch_pdl_cluster(group_kernel, GR_CLUSTER, dim3(warps * 32), smem, stream, ga);
+    return launch_pdl(group_kernel, dim3(1), dim3(warps * 32), smem, stream, ga);
 }
 
 }  // namespace
@@ -540,7 +564,7 @@ extern "C" int salt_b200_route_experts(const SaltB200RouteSpec* spec, const void
     a.sigmoid = s.scoring == SALT_B200_SCORE_SIGMOID; a.groups = s.n_groups; a.topk_groups = s.topk_groups; a.group_top = s.group_top;
     a.renormalize = s.renormalize != 0; a.scale = s.scale; a.bias = d_bias; a.selected = d_selected; a.weights = d_weights;
     if (a.groups == a.topk_groups) a.groups = a.topk_groups = 1;     // every group stays
-    GroupArgs g = {d_selected, rows * s.topk, s.n_experts, d_group_offsets, d_grouped_to_canonical, d_canonical_to_grouped};
+    GroupArgs g = {d_selected, rows * s.topk, s.n_experts, d_group_offsets, d_grouped_to_canonical, d_canonical_to_grouped, 0};
     const cudaStream_t st = (cudaStream_t)stream;
     const GroupArgs* gp = group ? &g : nullptr;
     cudaError_t e;
