@@ -168,12 +168,16 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         while (share * 2 * a.groups <= 32) share *= 2;
         const int g = lane / share, sub = lane - g * share;
         K k1 = 0, k2 = 0;
-        if (g < a.groups)
+        if (g < a.groups) {
+            int at = (g * share) % per + sub;            // each group from another place: groups of 32 would meet in the same banks
             for (int j = sub; j < per; j += share) {
-                const K k = keys[g * per + j];
+                if (at >= per) at -= per;
+                const K k = keys[g * per + at];
+                at += share;
                 k2 = max(k2, min(k1, k));
                 k1 = max(k1, k);
             }
+        }
         for (int d = 1; d < share; d <<= 1) {
             const K o1 = __shfl_xor_sync(FULL, k1, d), o2 = __shfl_xor_sync(FULL, k2, d);
             k2 = max(max(k2, o2), min(k1, o1));
