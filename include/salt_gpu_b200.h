@@ -593,8 +593,8 @@ int salt_b200_q4_expert_chain_static(const void *d_gate_vals, const void *d_gate
  *
  * Every call is asynchronous on `stream` (a cudaStream_t, NULL = default stream), keeps nothing between calls, allocates
  * nothing and may be captured; only weights_create / _destroy / _status allocate or synchronise.  All pointers are memory of the
- * current device unless stated; strides count elements.  0 = accepted, -1 = refused before anything was launched.  One
- * calling thread at a time. */
+ * current device unless stated; strides count elements; an output must not overlap an input.  0 = accepted, -1 = refused before
+ * anything was launched.  One calling thread at a time; weights_create, _destroy and _status not while it captures. */
 #define SALT_B200_F32 0
 #define SALT_B200_BF16 1
 #define SALT_B200_F16 2
@@ -639,7 +639,8 @@ int salt_b200_mxfp4_quantize(const void *d_x, int dtype, size_t row_stride, int 
 #define SALT_B200_ACT_GELU_TANH 1
 #define SALT_B200_ACT_SILU 2
 /* Matrices [rows][cols] of n_experts experts (1: a dense projection).  Pointers are HOST or device memory; they are read on
- * `stream` before create returns and not kept: the handle holds its own copy, laid out once for the kernels.  codes
+ * `stream` before create returns and not kept: the handle holds its own copy, laid out once for the kernels in tiles of 128 rows and 256
+ * columns (17 KB each; a gated pair's rows count together).  codes
  * [n_experts][rows][cols / 2], scales [n_experts][rows][cols / 32]; strides in bytes, 0 = dense.  With up_codes and up_scales (same
  * strides) the pair is gated: a product returns activation(gate row) * up row, and activation must be one of the two
  * functions.  A handle belongs to the device that is current when it is made; calls on another device are refused. */

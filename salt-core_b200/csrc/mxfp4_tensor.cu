@@ -56,7 +56,7 @@ struct MxTensorArgs {
     int cap;                             // most rows of a pass, a multiple of 16
     int stages, stage_bytes;
     uint32_t tmem_cols, acc_cols;        // columns of TMEM, and of one of the two accumulators at its start
-    int staged;                          // results go through shared memory behind the ring (long passes, rows that begin on 16 bytes)
+    int staged;                          // results go through shared memory behind the ring
     int split, share;                    // blocks of a cluster that share a unit, and most of its chunks that one takes
 };
 
@@ -670,19 +670,27 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     }
     // Two blocks per SM where there is work for them or where half the stages hold all chunks; otherwise one with twice the stages
     const bool pairs = small && (units * a.split > sms || a.share <= half);
-    const int blocks = pairs ? 2 * sms : sms;
-    a.stages = std::min(a.share, pairs ? half : std::min(MT_MAX_STAGES, (MT_SMEM - 1024) / a.stage_bytes));
-    if (a.split > 1) a.stages = std::max(a.stages, (a.cap * MX_TILE_ROWS * 4 + a.stage_bytes - 1) / a.stage_bytes);    // partial sums
-    int grid = a.split > 1 ? (int)units * a.split : (int)std::min<long long>(blocks, units);
     const bool pair = !small && a.split == 1 && w.row_tiles > 1;
     const size_t y_size = float_type_size(c.y_type);
+    // Results of long passes go through shared memory (4096 rows of 5120 x 5120: 48.5 -> 46.7 us); of short ones it costs what it
+    // saves (4096 of 5000 x 256: 17.6 and 19.0 us).
     a.staged = !small && a.split == 1 && (uintptr_t)c.y % 16 == 0 && c.y_stride * y_size % 16 == 0;
     const int slab = a.staged ? MT_BOX * MX_TILE_ROWS / (w.activation ? 2 : 1) * (int)y_size : 0;
+    long long turns = 1;                                 // units of a block
+    int grid = (int)units * a.split;
     if (pair) {
+        const long long two = passes * ((w.row_tiles + 1) / 2);
         a.stage_bytes = MX_TILE_BYTES + (a.cap / 2 + MT_BOX - 1) / MT_BOX * MT_BOX * MT_CHUNK + MT_SFB_BYTES;
-        grid = 2 * (int)std::min<long long>(sms / 2, passes * ((w.row_tiles + 1) / 2));
+        grid = 2 * (int)std::min<long long>(sms / 2, two);
+        turns = (two + grid / 2 - 1) / (grid / 2);
+    } else if (a.split == 1) {
+        grid = (int)std::min<long long>(pairs ? 2 * sms : sms, units);
+        turns = (units + grid - 1) / grid;
     }
-    if (!small && a.split == 1) a.stages = std::min(w.chunks, std::min(MT_MAX_STAGES, (MT_SMEM - 1024 - slab) / a.stage_bytes));
+    // as many stages as fit, but no more than a block has chunks
+    const int fit = std::min(MT_MAX_STAGES, ((pairs ? MT_SMALL_SMEM : MT_SMEM) - 1024 - slab) / a.stage_bytes);
+    a.stages = (int)std::min<long long>(fit, turns * a.share);
+    if (a.split > 1) a.stages = std::max(a.stages, (a.cap * MX_TILE_ROWS * 4 + a.stage_bytes - 1) / a.stage_bytes);    // partial sums
     const size_t smem = (size_t)a.stages * a.stage_bytes + slab + 1024;
     const auto kernel = pick_kernel(w.activation != 0, c.y_type, pair);
     if ((e = ensure_dynamic_smem((const void*)kernel, smem)) != cudaSuccess) return e;
