@@ -463,3 +463,78 @@ def test_rows_beyond_32_bits():
     eo.close(y[at].double().cpu().numpy(), want, err, "f32")
     y[at] = 0
     assert not y.any()
+
+
+def coded(seed, n, C):
+    """Random codes and scales as activations, and the values they stand for."""
+    rng = np.random.default_rng(seed)
+    code, byte = weights(rng, n, C)
+    held = np.full((n, eo.scale_pitch(C)), 0xff, np.uint8)               # the bytes behind the blocks are not read
+    held[:, :C // 32] = byte
+    return device(eo.mx_pack(code)), device(held), eo.mx_values(code, byte)
+
+
+# (rows, R, C, activation, groups or None, runs on pairs of SMs): shapes that reach the launch forms of long passes
+LONG = [(770, 1300, 5056, None, None, True), (800, 700, 5024, "silu", None, False), (2000, 1030, 5024, "silu", None, True),
+        (1537, 1409, 4000, "gelu_tanh", None, True), (1001, 2817, 2848, None, None, True),
+        (1500, 130, 7968, "gelu_tanh", None, False), (3000, 5000, 1056, None, None, False),
+        (97, 1, 8032, None, None, False), (300, 100, 8032, None, None, False), (150, 60, 5440, "silu", None, False),
+        (18889, 64, 1408, None, None, False), (20000, 100, 1440, None, None, False), (19000, 50, 1408, "silu", None, False),
+        (2600, 1300, 1568, None, [700, 0, 224, 225, 226, 900, 1, 324], True), (2600, 650, 1568, "silu", [0, 2600, 0, 0, 0, 0, 0, 0], True),
+        (14967, 64, 1376, None, [7000, 0, 7967], False)]
+
+
+@pytest.mark.parametrize("n,R,C,activation,groups,pair", LONG)
+@pytest.mark.parametrize("y_dtype,y_pad", [("bf16", 0), ("f32", 3), ("f16", 8)])
+def test_long_passes(n, R, C, activation, groups, pair, y_dtype, y_pad):
+    import torch
+    from graph_util import captured_kernels
+    counts = groups or [n]
+    E = len(counts)
+    held = Held(R + C, E, R, C, activation)
+    offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+    codes, scales, xv = coded(n, n, C)
+    off, y = device(offsets), torch.full((n + 1, R + y_pad), 55.0, dtype=tt(y_dtype), device="cuda")
+    torch.cuda.synchronize()
+
+    def call(stream=0):
+        if groups:
+            rc = held.handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), n, y.data_ptr(), y_dtype=y_dtype, y_row_stride=R + y_pad,
+                                     stream=stream)
+        else:
+            rc = held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr(), y_dtype=y_dtype, y_row_stride=R + y_pad, stream=stream)
+        assert rc == 0
+    call()
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    got = y.double().cpu().numpy()
+    assert (got[n:] == 55.0).all() and (got[:, R:] == 55.0).all()
+    for e in range(E):
+        b, t = offsets[e], offsets[e + 1]
+        if t > b:
+            want, err = held.want(xv[b:t], e)
+            eo.close(got[b:t, :R], want, err, y_dtype, f"group {e}")
+    (name, grid), = captured_kernels(call)
+    assert ("ELb1EEEv" in name) == pair, (name, grid)
+
+
+def test_pairs_repeat_their_bits():
+    """Long passes, twice in a row, on a busy chip and captured: the same bits."""
+    import torch
+    n, R, C = 1001, 2817, 2848
+    held = Held(5, 1, R, C)
+    codes, scales, _ = coded(1, n, C)
+    ys = [torch.empty(n, R, device="cuda") for _ in range(6)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i, y in enumerate(ys[:5]):
+        assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, y.data_ptr(), stream=streams[i % 2].cuda_stream) == 0
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        assert held.handle.matmul(codes.data_ptr(), scales.data_ptr(), n, ys[5].data_ptr(), stream=torch.cuda.current_stream().cuda_stream) == 0
+    g.replay()
+    torch.cuda.synchronize()
+    assert held.handle.status() == 0
+    for y in ys[1:]:
+        assert torch.equal(y, ys[0])
