@@ -12,8 +12,8 @@
 //
 // One warp per token: lane l holds experts l, l + 32, ...; the running maximum of the top-k is a warp-wide integer reduction of
 // order-preserving bit patterns.  Bound by the chain of reductions (two per selected expert), not by memory: 4099 tokens of 256
-// experts 8.1 us (plain softmax) and 15 us (sigmoid, bias, eight groups); grouping their 32 792 selections 8 us more, mostly one
-// cluster's scattered 4-byte stores.  One token of 128 experts, routed and grouped in one launch: 4 us.
+// experts 8.1 us (plain softmax) and 14.6 us (sigmoid, bias, eight groups; 2 of them rows done again); grouping their 32 792 selections
+// 7.5 us more, a dozen synchronised phases of one cluster.  One token of 128 experts, routed and grouped in one launch: 4 us.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
