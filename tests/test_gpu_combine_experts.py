@@ -90,3 +90,17 @@ def test_offsets_beyond_32_bits():
     y = torch.empty(1, 64, device="cuda")
     assert ex.combine(rows.data_ptr(), n, 64, idx.data_ptr(), w.data_ptr(), 1, 2, y.data_ptr(), dtype="bf16", row_stride=stride) == 0
     assert torch.equal(y[0].cpu(), torch.arange(64.0))
+
+
+def test_no_rows():
+    """Tokens none of whose rows exist are zeros, also where there are no rows at all."""
+    import torch
+    for cols in (64, 37):
+        y = torch.full((3, cols), 55.0, device="cuda")
+        idx = torch.full((6,), -1, dtype=torch.int32, device="cuda")
+        w = torch.ones(6, device="cuda")
+        assert ex.combine(0, 0, cols, idx.data_ptr(), w.data_ptr(), 3, 2, y.data_ptr()) == 0
+        assert not y.any()
+        y.fill_(55.0)
+        assert ex.combine(0, 0, cols, 0, w.data_ptr(), 3, 2, y.data_ptr()) == 0
+        assert not y.any()

@@ -538,3 +538,39 @@ def test_pairs_repeat_their_bits():
     assert held.handle.status() == 0
     for y in ys[1:]:
         assert torch.equal(y, ys[0])
+
+
+@pytest.mark.parametrize("activation", [None, "silu"])
+def test_host_weights_of_several_experts_and_a_single_group(activation):
+    """Weights from host memory, gone after the handle is made; and a handle of one expert called by groups."""
+    import gc
+    import torch
+    for E, counts in ((3, [2, 0, 70]), (1, [45])):
+        held = Held(60 + E, E, 140, 544, activation, host=True)
+        gc.collect()
+        offsets = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+        n = int(offsets[-1])
+        codes, scales, xv = acts(n, n, 544, "f16")
+        off, y = device(offsets), torch.empty(n, 140, device="cuda")
+        torch.cuda.synchronize()
+        assert held.handle.experts(codes.data_ptr(), scales.data_ptr(), off.data_ptr(), n, y.data_ptr()) == 0
+        got = y.double().cpu().numpy()
+        for e in range(E):
+            b, t = offsets[e], offsets[e + 1]
+            if t > b:
+                want, err = held.want(xv[b:t], e)
+                eo.close(got[b:t], want, err, "f32", f"expert {e} of {E}")
+
+
+def test_weights_of_quantized_rows():
+    """Weights quantised on the device, their scale rows as the quantiser leaves them, straight into a handle."""
+    import torch
+    R, C, n = 300, 1056, 19
+    w = torch.randn(R, C, device="cuda").bfloat16() / 32
+    codes, scales, _ = quantize(w, "bf16")
+    handle = ex.Mxfp4Weights(R, C, 1, codes.data_ptr(), scales.data_ptr(), scale_row_stride=eo.scale_pitch(C))
+    xc, xs, xv = acts(2, n, C, "bf16")
+    y = torch.empty(n, R, device="cuda")
+    assert handle.matmul(xc.data_ptr(), xs.data_ptr(), n, y.data_ptr()) == 0
+    want, err = eo.product(xv, eo.mx_values(*eo.mx_quantize(w.double().cpu().numpy())))
+    eo.close(y.double().cpu().numpy(), want, err, "f32")
