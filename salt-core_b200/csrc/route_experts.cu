@@ -185,27 +185,33 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         }
         __syncwarp();
         K mine = k1;
-        if (a.group_top == 2 && k1 && k2) mine = Q::of(Q::value(k1) + Q::value(k2));
-        if (g >= a.groups || sub != 0) mine = 0;
-        uint32_t stay = 0;                               // bit g: the group stays
-        K last = 0;
-        bool decided = true;
-        for (int r = 0; r <= a.topk_groups; r++) {
-            int at;
-            const K m = Q::best(mine, g, at);
-            if (!m) break;
-            if (r == a.topk_groups) {                    // the best group that goes
-                if (!wide && !by_logit) {
-                    const S x = Q::value(last), y = Q::value(m);
-                    decided = x - y > (S)2 * slack + (S)4e-7 * (fabs(x) + fabs(y));
-                }
-                break;
+        S far = 0;                                       // how far the sum may be from that of the exact keys; each is rounded in units
+        if (g >= a.groups || sub != 0) mine = 0;         // of its own size, which the sum does not show where two of them cancel
+        if (mine) {
+            const S x = Q::value(k1);
+            far = (S)2 * slack + (S)4e-7 * fabs(x);
+            if (a.group_top == 2 && k2) {
+                const S y = Q::value(k2);
+                far += (S)4e-7 * fabs(y);
+                mine = Q::of(x + y);
             }
-            stay |= 1u << at;
-            last = m;
-            if (g == at) mine = 0;
         }
-        if (!decided) return false;
+        uint32_t stay = 0;                               // bit g: the group stays
+        K left = mine;
+        for (int r = 0; r < a.topk_groups; r++) {
+            int at;
+            if (!Q::best(left, g, at)) break;
+            stay |= 1u << at;
+            if (g == at) left = 0;
+        }
+        if (!wide && !by_logit) {
+            // decided if the least that a staying group can be worth is above the most that any other can
+            const float v = mine ? (float)Q::value(mine) : 0.f, low = v - (float)far;
+            const bool stays = mine != left;
+            const uint32_t l = !stays ? 0xffffffffu : ordered(low > -CUDART_INF_F ? low : -CUDART_INF_F);       // false for NaN
+            const float least = Keys<float>::value(__reduce_min_sync(FULL, l));
+            if (__any_sync(FULL, left && !(v + (float)far < least))) return false;
+        }
         const uint32_t inverse = ((1u << 20) + per - 1) / per;       // e / per for e * per below 2^20
 #pragma unroll
         for (int i = 0; i < VPT; i++) {

@@ -1,0 +1,30 @@
+"""Routing where 32 bits come close to deciding wrongly: sums of group keys that cancel, biases of the lowest and the largest value,
+scores far below one.  Against the statement in 64 bits."""
+import numpy as np
+import pytest
+
+import expert_ops_oracle as eo
+from test_gpu_route_experts import check, logits_of, run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("G,h", [(32, 0.5), (32, 1.5), (32, 4.5), (16, 20.0), (24, 300.0)])
+def test_group_sums_that_cancel(scoring, G, h):
+    """Groups of two experts with biases of +h and -h: a key is rounded to a unit of h, their sum is as small as the scores."""
+    keep = G // 2
+    bias = h * np.where(np.arange(2 * G) % 2, -1.0, 1.0)
+    check(logits_of(int(8 * h) + G, 3000, 2 * G, "f32", 0.01), 2 * keep, bias=bias, scoring=scoring, n_groups=G, topk_groups=keep, group_top=2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_one_group_of_large_keys_among_small_ones(scoring):
+    """Only some groups have keys far larger than their sums; they stay or go beside groups whose keys are exact to their last bits."""
+    G, per = 16, 4
+    bias = np.zeros((G, per))
+    for g in (1, 4, 5, 9, 14):
+        bias[g] = [37.0, -37.0, -80.0, -80.0]
+    bias[7] = [3e30, -3e30, -3.2e38, -3.2e38]
+    check(logits_of(12, 3000, G * per, "f32", 0.02), 8, bias=bias.reshape(-1), scoring=scoring, n_groups=G, topk_groups=8,
+          group_top=2, renormalize=False)
