@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <float.h>
 #include <limits.h>
 
 #include <algorithm>
@@ -194,6 +195,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
                 const S y = Q::value(k2);
                 far += (S)4e-7 * fabs(y);
                 mine = Q::of(x + y);
+                mine = max(mine, (K)1);                  // two of the lowest value: no sum in 32 bits, but a group that can stay
             }
         }
         uint32_t stay = 0;                               // bit g: the group stays
@@ -206,7 +208,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         }
         if (!wide && !by_logit) {
             // decided if the least that a staying group can be worth is above the most that any other can
-            const float v = mine ? (float)Q::value(mine) : 0.f, low = v - (float)far;
+            const float v = mine > 1 ? (float)Q::value(mine) : -FLT_MAX, low = mine > 1 ? v - (float)far : -CUDART_INF_F;
             const bool stays = mine != left;
             const uint32_t l = !stays ? 0xffffffffu : ordered(low > -CUDART_INF_F ? low : -CUDART_INF_F);       // false for NaN
             const float least = Keys<float>::value(__reduce_min_sync(FULL, l));

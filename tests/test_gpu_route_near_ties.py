@@ -28,3 +28,19 @@ def test_one_group_of_large_keys_among_small_ones(scoring):
     bias[7] = [3e30, -3e30, -3.2e38, -3.2e38]
     check(logits_of(12, 3000, G * per, "f32", 0.02), 8, bias=bias.reshape(-1), scoring=scoring, n_groups=G, topk_groups=8,
           group_top=2, renormalize=False)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("keep", [1, 3, 6])
+@pytest.mark.parametrize("top", [1, 2])
+def test_biases_of_the_lowest_and_the_largest_value(scoring, keep, top):
+    """A bias of the type's lowest value is a mask that still orders: two such keys add up to less than 32 bits hold, and their group
+    is still one that can stay.  The same with the largest value."""
+    low, high = np.finfo(np.float32).min, np.finfo(np.float32).max
+    per, E = 4, 32
+    for masked in (range(4, 32), range(0, 28), range(0, 32), [0, 1, 2, 3, 9, 10, 11, 17, 18, 24]):
+        bias = np.linspace(-0.1, 0.1, E)
+        bias[list(masked)] = low
+        check(logits_of(5, 40, E, "f32"), 4, bias=bias, scoring=scoring, n_groups=8, topk_groups=keep, group_top=top)
+        bias[[2, 3, 12, 13, 14, 21]] = high
+        check(logits_of(6, 40, E, "f32"), 4, bias=bias, scoring=scoring, n_groups=8, topk_groups=keep, group_top=top)
+
+
