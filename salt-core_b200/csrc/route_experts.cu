@@ -116,6 +116,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
     constexpr bool wide = sizeof(S) == 8;
     S score[VPT];
     S top_score = 1;                                     // no score is larger
+    float m = 0.f;                                       // a score is about exp(l - m) where it is small
     if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < VPT; i++) {
@@ -124,7 +125,7 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
             score[i] = Q::quotient(x < (S)0 ? t : (S)1, (S)1 + t);
         }
     } else {
-        float m = -CUDART_INF_F;
+        m = -CUDART_INF_F;
 #pragma unroll
         for (int i = 0; i < VPT; i++) m = fmaxf(m, l[i]);            // fmaxf passes over NaN
         m = Keys<float>::value(__reduce_max_sync(FULL, max(Keys<float>::of(m), 1u)));
@@ -249,6 +250,14 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
                 if (!((taken >> i) & 1u) && key[i] > mine) { mine = key[i]; at_i = i; }
         }
     }
+    if (!wide && (a.bias || (float)Q::value(last) - m < -60.f)) {       // without a bias the last one has the lowest logit
+        // A score that 32 bits hold with few bits or not at all can become an ordinary weight, by the sum of the selected ones or by
+        // the scale.  Below exp(-800) it is zero in 64 bits, too.
+        bool faint = false;
+#pragma unroll
+        for (int i = 0; i < VPT; i++) faint |= ((taken >> i) & 1u) && score[i] < (S)1e-30 && l[i] - m > -800.f;
+        if (__any_sync(FULL, faint)) return false;
+    }
     S div = 1;
     if (a.renormalize) {
         S sum = 0;
@@ -256,7 +265,6 @@ __device__ bool route_token(const RouteArgs& a, const float (&l)[VPT], int token
         for (int i = 0; i < VPT; i++)
             if ((taken >> i) & 1u) sum += score[i];
         sum = warp_sum(sum);
-        if (!wide && !(sum > (S)1e-30) && found) return false;       // too small for 32 bits
         div = sum > (S)0 ? sum : (S)1;
     }
     int32_t* ids = a.selected + (size_t)token * a.topk;

@@ -44,3 +44,29 @@ def test_biases_of_the_lowest_and_the_largest_value(scoring, keep, top):
         check(logits_of(6, 40, E, "f32"), 4, bias=bias, scoring=scoring, n_groups=8, topk_groups=keep, group_top=top)
 
 
+@pytest.mark.parametrize("bias", [None, "masks"])
+@pytest.mark.parametrize("scoring,renorm,scale", [("sigmoid", True, 1.0), ("sigmoid", False, 1e30), ("softmax", True, 1e30), ("softmax", False, 1e25)])
+def test_weights_of_scores_below_32_bits(scoring, renorm, scale, bias):
+    """Selected scores that 32 bits hold with few bits or not at all: their weights, brought back by the sum or the scale, are those
+    of 64 bits.  A score is off by less than 2^-45 there, so half a step of the result is all that is left."""
+    import torch
+    E = 40
+    l = torch.full((6, E), -400.0)
+    l[0, :4] = torch.tensor([-66.0, -88.5, -95.0, -101.0])
+    l[1, :4] = torch.tensor([0.0, -90.25, -103.0, -110.0])
+    l[2, 5:9] = torch.tensor([0.0, -60.0, -75.0, -1000.0])
+    l[3, 30:] = torch.linspace(-120, -84, 10)
+    l[4] = torch.linspace(-3, 3, E)
+    l[5, 7] = 4.0
+    l[5, 8:12] = -98.0
+    b = None if bias is None else np.where(np.arange(E) % 13 == 12, np.finfo(np.float32).min, 0.0)
+    sel, w, *_ = run(l.cuda(), 4, bias=b, scoring=scoring, renormalize=renorm, scale=scale)
+    want, ww = eo.route(l.double().numpy(), 4, bias=b, scoring=scoring, renormalize=renorm, scale=float(np.float32(scale)))
+    assert np.array_equal(sel, want)
+    # Rows whose selected scores are all above 1e-30 are held in 32 bits with all their bits (row 3 of a softmax: e^-12 and more of the
+    # largest): 110 roundings as in test_gpu_route_experts.check.  The others are done in 64.
+    _, scores = eo.route(l.double().numpy(), 4, bias=b, scoring=scoring, renormalize=False)
+    small = scores.min(axis=1) < 1e-30
+    assert small[[1, 2, 5]].all() and not small[4]
+    eo.close(w[small], ww[small], 2.0 ** -45 * ww[small], "f32")
+    eo.close(w[~small], ww[~small], 110 * 2.0 ** -24 * ww[~small], "f32")
