@@ -659,7 +659,8 @@ int salt_b200_mxfp4_matmul(void *weights, const uint8_t *d_codes, const uint8_t 
  * those of expert e; rows in no group keep what d_y held.  `rows` bounds the rows that are read and written. */
 int salt_b200_mxfp4_experts(void *weights, const uint8_t *d_codes, const uint8_t *d_scales, const int32_t *d_group_offsets,
                             int rows, void *d_y, int y_dtype, size_t y_row_stride, void *stream);
-/* Synchronise `stream`, read and clear the handle's device error word.  0 = clean, -1 = refused or failed. */
+/* Synchronise `stream`, read and clear the handle's device error word.  0 = clean, -1 = refused, or a product of this handle gave
+ * up a wait since the last call and its results are not whole. */
 int salt_b200_mxfp4_status(void *weights, void *stream);
 
 /* d_y[t] = sum over j of d_weights[t * topk + j] * d_rows[d_row_index[t * topk + j]], j ascending, in 32 bits, rounded once;

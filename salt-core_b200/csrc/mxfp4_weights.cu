@@ -170,7 +170,7 @@ int salt_b200_mxfp4_status(void* weights, void* stream) {
         !cuda_ok(cudaMemsetAsync(w->status, 0, sizeof(int), (cudaStream_t)stream), "mxfp4 status") ||
         !cuda_ok(cudaStreamSynchronize((cudaStream_t)stream), "mxfp4 status"))
         return -1;
-    return status;
+    return status ? -1 : 0;
 }
 
 }  // extern "C"

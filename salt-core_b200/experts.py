@@ -101,6 +101,7 @@ class Mxfp4Weights:
                                                 self.rows if y_row_stride is None else y_row_stride, stream)
 
     def status(self, stream=0):
+        """0 where every product so far is whole, -1 after one that gave up (or a refused call); reading clears it."""
         return self.lib.salt_b200_mxfp4_status(self.handle, stream)
 
     def close(self):
