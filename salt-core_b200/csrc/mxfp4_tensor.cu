@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             for (uint32_t t = produced > n ? produced - n : 0; t < produced; t++) (void)mbar_wait(&bar_full[t % n], (t / n) & 1, &none);
         }
         __syncthreads();
-        if (warp == 8 && lane == 0 && (!PAIR || rank == 0)) {
+        if (warp == 8 && (!PAIR || rank == 0) && elected()) {        // the lane that issued the MMAs: a commit covers its own only
             int none = 0;
             if (PAIR)
                 asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&bar_drain)) : "memory");
