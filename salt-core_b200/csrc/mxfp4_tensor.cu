@@ -707,6 +707,11 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     const int fit = std::min(MT_MAX_STAGES, ((pairs ? MT_SMALL_SMEM : MT_SMEM) - 1024 - slab) / a.stage_bytes);
     a.stages = (int)std::min<long long>(fit, turns * a.share);
     if (a.split > 1) a.stages = std::max(a.stages, (a.cap * MX_TILE_ROWS * 4 + a.stage_bytes - 1) / a.stage_bytes);    // partial sums
+    // Blocks that wait for one another hold TMEM while they do, and one that finds none left waits for it without a limit; of two such
+    // groups on the same SMs, each could hold what the other waits for.  None can be: a block of a pair, or of a cluster that takes all
+    // of TMEM, comes with long rows only and asks for 167 KB and more of an SM's 228, one of a cluster that takes half of it for 47 and
+    // more, and each has 10 KB beside that (the least that the rules above give, over 1.3 million sizes).  A rule that changes this must
+    // ask for more here.
     const size_t smem = (size_t)a.stages * a.stage_bytes + slab + 1024;
     const auto kernel = pick_kernel(w.activation != 0, c.y_type, pair);
     if ((e = ensure_dynamic_smem((const void*)kernel, smem)) != cudaSuccess) return e;

@@ -15,6 +15,11 @@ def _ok(rc, what):
 
 def captured_kernels(call):
     """[(name, grid)] of the kernels that `call(stream)` launches on `stream`; it is run once before, uncaptured (set-up)."""
+    return [(name, grid) for name, grid, _ in captured_launches(call)]
+
+
+def captured_launches(call):
+    """The same with the dynamic shared memory of a block: [(name, grid, bytes)]."""
     import torch
     cu = C.CDLL("libcuda.so.1")
     stream = torch.cuda.Stream()
@@ -44,6 +49,6 @@ def captured_kernels(call):
             _ok(cu.cuKernelGetName(C.byref(name), C.c_void_p(p.kern)), "kernel name")
         else:
             _ok(cu.cuFuncGetName(C.byref(name), C.c_void_p(p.func)), "function name")
-        found.append((name.value.decode(), tuple(p.grid)))
+        found.append((name.value.decode(), tuple(p.grid), p.shared))
     _ok(cu.cuGraphDestroy(graph), "destroy")
     return found
