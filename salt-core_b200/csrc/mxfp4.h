@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "mxfp4_passes.h"
+
 namespace sb {
 
 // Layout made once at creation: per 128 stored rows and 256 columns one tile of 17 KB that a single bulk copy brings into shared
@@ -12,10 +14,7 @@ namespace sb {
 //   1024 bytes of scales: block c of row r at (c / 4) * 512 + (r % 32) * 16 + (r / 32) * 4 + c % 4.
 // A gated pair is stored with its rows alternating (gate row i at 2 i, up row i at 2 i + 1), so that the two values an activation
 // needs lie side by side in every kernel.  Rows and columns that fill a tile up have codes 0 and scales 127 = 2^0.
-constexpr int MX_TILE_ROWS = 128, MX_TILE_COLS = 256;
-constexpr int MX_CODE_BYTES = MX_TILE_ROWS * MX_TILE_COLS / 2;
-constexpr int MX_TILE_BYTES = MX_CODE_BYTES + MX_TILE_ROWS * MX_TILE_COLS / 32;
-
+// (The sizes are in mxfp4_passes.h.)
 struct Mxfp4Weights {
     int device;
     int rows, cols, experts;     // rows of the result; cols = K

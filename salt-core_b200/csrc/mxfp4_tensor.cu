@@ -25,12 +25,12 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cmath>
 
 #include "../../include/salt_gpu_b200.h"
 #include "float_types.cuh"
 #include "internal.h"
 #include "mxfp4.h"
+#include "mxfp4_passes.h"
 #include "pdl.cuh"
 #include "umma.cuh"
 
@@ -40,10 +40,6 @@ namespace sb {
 namespace {
 
 constexpr int MT_THREADS = 320;          // warps 0-3 scales, 4-7 epilogue, 8 issuer, 9 producer
-constexpr int MT_CHUNK = 128;            // packed bytes of a K chunk
-constexpr int MT_BOX = 32;               // rows of an activation copy
-constexpr int MT_MAX_N = 224;            // two accumulators of 224 columns and 64 columns of scales fill TMEM
-constexpr int MT_SMALL_N = 96;           // two of 96 columns and the scales half of it: two blocks per SM
 constexpr uint32_t MT_SF_STRIDE = 32, MT_SFB = 8;
 constexpr int MT_SFB_BYTES = 2048;
 constexpr int MT_MAX_STAGES = 8;
@@ -134,12 +130,6 @@ __device__ __forceinline__ bool epilogue_agrees(bool ok) {
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 struct Unit { int expert, tile, row0, n, N; };   // n rows of the pass, N = n up to a multiple of 16
-
-// Passes of a group of n rows: as few as the cap allows, of equal size up to the multiple of 16.
-__host__ __device__ __forceinline__ int pass_rows(int n, int cap) {
-    const int passes = (n + cap - 1) / cap;
-    return passes ? ((n + passes - 1) / passes + 15) & ~15 : cap;
-}
 
 struct Groups {
     const int *first, *begin;            // [experts + 1] passes before a group and its first row (shared memory); null for one dense matrix
@@ -602,34 +592,6 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
     }
-}
-
-// Most rows of a pass, for `groups` groups that are expected to have `rows` rows (of expert groups a quarter and 8 above the average:
-// a longer one takes a pass more, which reads its weights again, from L2).  Longer passes load less in all; shorter ones keep more
-// SMs busy, write their results sooner, and up to 96 rows two blocks share an SM.  Microseconds by what was measured: a chunk takes a
-// block 0.3, or 0.4 with a second one beside it, a column of results 0.022, and all SMs together load 11 TB/s from L2.  64
-// experts of 1536 x 5120, 16 / 31 / 63 rows on average: 58 / 89 / 93 us by passes of up to 96, 65 / 99 / 104 by longer ones; 125
-// rows: 130 and 111.
-int choose_cap(int rows, int groups, int row_tiles, int chunks, int sms) {
-    int best = 0;
-    double least = 0, fewest = 0;
-    for (int cap = MT_BOX; cap <= MT_MAX_N; cap += MT_BOX) {
-        const double passes = (double)groups * ((rows + cap - 1) / cap), units = passes * row_tiles;
-        const int n = pass_rows(rows, cap);
-        const bool two = cap <= MT_SMALL_N && units > sms;
-        const double rounds = std::ceil(units / (two ? 2 * sms : sms)), loop = chunks * (two ? 0.4 : 0.3), store = 0.022 * n;
-        const double loads = units * chunks * (MX_TILE_BYTES + (cap > MT_SMALL_N ? n / 2 : n) * MT_CHUNK) / 11e6;
-        const double t = std::max(rounds * std::max(loop, store) + std::min(loop, store), loads);
-        // as many passes by more room for them: no gain; a tenth is within what the estimate leaves out (37 rows of 2112 x 2816: 6.4 us
-        // in one pass, 7.1 in two)
-        if (!best || (passes < fewest && t < 1.1 * least)) {
-            best = cap;
-            least = t;
-            fewest = passes;
-        }
-        if (cap >= rows) break;
-    }
-    return best;
 }
 
 using Kernel = void (*)(const MxTensorArgs, const CUtensorMap);
