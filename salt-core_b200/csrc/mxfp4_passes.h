@@ -18,6 +18,7 @@ constexpr int MX_TILE_BYTES = MX_CODE_BYTES + MX_TILE_ROWS * MX_TILE_COLS / 32;
 constexpr int MT_CHUNK = 128;            // packed bytes of a K chunk
 constexpr int MT_BOX = 32;               // rows of an activation copy
 constexpr int MT_MAX_N = 224;            // two accumulators of 224 columns and 64 columns of scales fill TMEM
+constexpr int MT_MAX_SPLIT = 8;
 constexpr int MT_SMALL_N = 96;           // two of 96 columns and the scales half of it: two blocks per SM
 
 // Passes of a group of n rows: as few as the cap allows, of equal size up to the multiple of 16.
@@ -59,6 +60,27 @@ inline int choose_cap(int rows, int groups, int row_tiles, int chunks, int sms) 
             best = cap;
             taken = t;
             fewest = passes;
+        }
+    }
+    return best;
+}
+
+// Blocks of a cluster that share a unit's chunks (1, 2, 4 or 8), where there are few units.  Two blocks fit on an SM where the share is
+// at most `half` chunks; 0: never.
+// Joining the parts costs about as much as four to six chunks of one block (0.33 us each); by 1 / 2 / 4 / 8 blocks one row of 2304 x 4096
+// takes 7.4 / 6.6 / 6.4 / 6.5 us, of 1920 x 16384 18.4 / 12.2 / 9.2 / 8.6 (32 units of 16 chunks are the exception: 7.5 / 6.8 / 7.2).
+// Units that wait for a place cost more than they save.  Blocks that fill an SM each find one for 74 clusters of two, 33 of four and 15
+// of eight among 148 SMs: 16 units of 64 chunks take 9.4 us by four and 13.4 by eight, 34 of them 13.6 by two and 18.8 by four; 130
+// blocks are within both smaller forms.  Two to an SM, 160 blocks still gain nothing and lose nothing (40 units of 16 chunks: 7.1 by
+// two, 7.3 by four), 256 of eight lose (36 units: 12.1).
+inline int choose_split(long long units, int chunks, int half, int sms) {
+    int best = 1, cost = chunks;
+    for (int split = 2; split <= MT_MAX_SPLIT; split *= 2) {
+        const int share = (chunks + split - 1) / split;
+        const int places = share <= half ? sms + sms / 12 : split == 8 ? sms * 13 / 16 : sms - sms / 8;
+        if (units * split <= places && share + 4 + split / 4 < cost) {
+            best = split;
+            cost = share + 4 + split / 4;
         }
     }
     return best;

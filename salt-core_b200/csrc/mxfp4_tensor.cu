@@ -43,7 +43,6 @@ constexpr int MT_THREADS = 320;          // warps 0-3 scales, 4-7 epilogue, 8 is
 constexpr uint32_t MT_SF_STRIDE = 32, MT_SFB = 8;
 constexpr int MT_SFB_BYTES = 2048;
 constexpr int MT_MAX_STAGES = 8;
-constexpr int MT_MAX_SPLIT = 8;
 constexpr int MT_SMEM = 217 * 1024, MT_SMALL_SMEM = 103 * 1024;
 
 struct MxTensorArgs {
@@ -630,22 +629,9 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     const long long passes = c.offsets ? std::min<long long>(c.rows, c.rows / a.cap + w.experts) : (c.rows + a.cap - 1) / a.cap;
     const long long units = passes * w.row_tiles;
     if (units > INT32_MAX / 2) return cudaErrorInvalidValue;
-    // Few units: a cluster shares each.  Joining the parts costs about as much as four to six chunks of one block (0.33 us each):
-    // 4096 x 4096, one row: 8.3 / 6.9 / 6.8 us by clusters of 1 / 2 / 4; 5120 x 1536, 32 rows: 4.8 / 6.4.  Blocks that wait for a
-    // place cost more than they save: 96 units of 20 chunks 13.1 / 13.8 / 19.6.  Clusters of blocks that fill an SM each do not
-    // cover all SMs (17 of eight blocks: 11.9 us against 6.2 for 17 of four).
     const int half = std::min(MT_MAX_STAGES, (MT_SMALL_SMEM - 1024) / a.stage_bytes);
-    a.split = 1;
-    a.share = w.chunks;
-    int cost = w.chunks;
-    for (int split = 2; split <= MT_MAX_SPLIT; split *= 2) {
-        const int share = (w.chunks + split - 1) / split, places = small && share <= half ? sms + sms / 12 : sms - sms / 8;
-        if (units * split <= places && share + 4 + split / 4 < cost) {
-            a.split = split;
-            a.share = share;
-            cost = share + 4 + split / 4;
-        }
-    }
+    a.split = choose_split(units, w.chunks, small ? half : 0, sms);
+    a.share = (w.chunks + a.split - 1) / a.split;
     // Two blocks per SM where there is work for them or where half the stages hold all chunks; otherwise one with twice the stages
     const bool pairs = small && (units * a.split > sms || a.share <= half);
     const bool pair = !small && a.split == 1 && w.row_tiles > 1;
