@@ -38,12 +38,17 @@ struct Mxfp4Call {
 // mxfp4_tensor.cu: any number of rows
 cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cudaStream_t stream);
 
-// y = act(gate) * up
+// y = act(gate) * up.  Both activations are g / (1 + exp(-z)): z = g is SiLU, z = 2 sqrt(2 / pi) (g + 0.044715 g^3) the tanh form of GELU.
+// With t = exp(-|z|) that is g / (1 + t) above zero and g t / (1 + t) below it: the quotient's divisor lies between 1 and 2, and a gate far
+// below zero keeps its bits until the result is too small for 32.  (exp(-z) as it stands grows past 2^126 there, where the fast
+// quotient is zero, and the fast exponential is off by |z| units; both together were 0.3 to 1.1 us faster: 64 experts of 1536 x 5120 for
+// 1999 tokens 104.9 -> 105.3, 4096 rows of 2560 x 5120 53.1 -> 53.9.)
 __device__ __forceinline__ float gate_act(int activation, float g) {
-    // both are g / (1 + exp(-z)): z = g is SiLU, z = 2 sqrt(2 / pi) (g + 0.044715 g^3) the tanh form of GELU.  The fast exponential and
-    // quotient are off by a few units of 2^-24 |z| where exp(-z) matters, which against |g| stays below 2^-21
     const float z = activation == 2 ? g : 1.5957691216057308f * (g + 0.044715f * g * g * g);
-    return __fdividef(g, 1.0f + __expf(-z));
+    const float t = expf(-fabsf(z));
+    float r;                                             // of a number from 1 to 2: one unit off at most, nothing to flush
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
+    return (z < 0.f ? g * t : g) * r;
 }
 
 // Bulk copy of a tile (both addresses on 16 bytes, a multiple of 16 bytes) into this block's own shared memory.
