@@ -194,7 +194,7 @@ extern "C" int salt_b200_mxfp4_quantize(const void* d_x, int dtype, size_t row_s
                                         void* d_values, void* stream) {
     using namespace sb;
     if (!float_type_ok(dtype) || cols < 32 || cols % 32 || cols > SALT_B200_MXFP4_MAX_COLS || rows < 0 || src_rows < 0 ||
-        index_div < 1 || row_stride < (size_t)cols || row_stride > (size_t)1 << 40 || (!d_row_index && rows > src_rows))
+        row_stride < (size_t)cols || row_stride > (size_t)1 << 40 || (d_row_index ? index_div < 1 : rows > src_rows))
         return -1;
     if (rows == 0) return 0;
     const size_t size = float_type_size(dtype);
