@@ -113,19 +113,8 @@ __device__ __forceinline__ bool elected() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(p));
     return p != 0;
 }
-// Barrier 1 among the four epilogue warps: true if all of them bring true.
-__device__ __forceinline__ bool epilogue_agrees(bool ok) {
-    uint32_t all;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 q, %1, 0;\n\t"
-        "bar.red.and.pred p, 1, 128, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(all)
-        : "r"((uint32_t)ok)
-        : "memory");
-    return all != 0;
-}
+// Barrier 1 among the four epilogue warps.
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 struct Unit { int expert, tile, row0, n, N; };   // n rows of the pass, N = n up to a multiple of 16
@@ -451,7 +440,8 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             pdl_wait();
             pdl_launch_dependents();
         }
-        for (int u = first_unit; u < units && ok; u += unit_step) {
+        int u = first_unit;
+        for (; u < units && ok; u += unit_step) {
             Unit un;
             if (!groups.unit(u, &un)) continue;
             if (kc0 >= kc1) continue;                    // this block of the cluster has no chunks
@@ -463,9 +453,6 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             const uint32_t buf = done & 1u;
             ok = mbar_wait(&bar_done[buf], (done >> 1) & 1, fail);
             ok = __all_sync(0xffffffffu, ok);
-            // Where results meet in shared memory the four warps go on together or not at all: a warp that has given up reaches no
-            // other barrier.  Behind this one the slab of the unit before has been stored.
-            if (a.staged) ok = epilogue_agrees(ok);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             for (int n0 = 0; n0 < un.N; n0 += 32) {
@@ -494,12 +481,12 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
                     }
                     if (stage_out) {
                         T* slab = (T*)(stage_base + a.stages * a.stage_bytes);
-                        if (n0 > 0) asm volatile("bar.sync 1, 128;" ::: "memory");       // the slab before this one has been stored
+                        epilogue_sync();                 // the slab before this one has been stored
 #pragma unroll
                         for (int k = 0; k < (GATED ? 16 : 32); k++)
                             if (GATED) slab[(2 * k + odd) * WIDTH + (q * 32 + lane) / 2] = out[k];
                             else slab[k * WIDTH + q * 32 + lane] = out[k];
-                        asm volatile("bar.sync 1, 128;" ::: "memory");
+                        epilogue_sync();
                         constexpr int PIECES = WIDTH * (int)sizeof(T) / 16;
                         T* y = (T*)a.c.y + (size_t)(un.row0 + n0) * a.c.y_stride + (m - q * 32 - lane) / (GATED ? 2 : 1);
                         const int pieces = min(32, un.n - n0) * PIECES;
@@ -531,6 +518,17 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             }
             done++;
         }
+        // Where results meet in shared memory a warp that has given up still comes to every barrier that the others may wait at, from
+        // the unit that it broke off.  (Four warps that agree at a barrier with a reduction cost 2 us of 63.)
+        if (!ok && a.staged)
+            for (; u < units; u += unit_step) {
+                Unit un;
+                if (!groups.unit(u, &un) || ((PAIR ? 2 * un.tile + rank : un.tile) + 1) * MX_TILE_ROWS > a.w.stored_rows) continue;
+                for (int n0 = 0; n0 < un.N; n0 += 32) {
+                    epilogue_sync();
+                    epilogue_sync();
+                }
+            }
     }
 
     if (!PAIR && a.split > 1) {
