@@ -585,15 +585,16 @@ int salt_b200_q4_expert_chain_static(const void *d_gate_vals, const void *d_gate
 
 /* ---- Experts without a stack -------------------------------------------------------------------------------------- */
 /* Operators on device pointers for a host that keeps its own layers: routing with scores, balance bias and expert groups,
- * MXFP4 (W4A4) quantisation and products, and the weighted combine.  No counterpart in the reference (its router is the
- * softmax top-k of models/gemma4-26b-a4b/src/gemma4.c:132-186, its four-bit formats are affine Q4 and NVFP4).
+ * MXFP4 (W4A4) quantisation and products, and the weighted combine.  The reference has parts of them as scalar CPU code: MXFP4
+ * kernels in src/kernels.c, a router whose biased score selects and whose unbiased scores weigh in src/router.c:22-57, and one
+ * of sigmoid scores with a bias in models/lfm2-24b-a2b/lfm_router.c:9-69.  No result here is bound to theirs bit for bit.
  *
  *   salt_b200_route_experts -> salt_b200_mxfp4_quantize (token rows in grouped order) -> salt_b200_mxfp4_experts (gate | up)
  *   -> salt_b200_mxfp4_quantize -> salt_b200_mxfp4_experts (down) -> salt_b200_combine_experts
  *
  * Every call is asynchronous on `stream` (a cudaStream_t, NULL = default stream), keeps nothing between calls, allocates
  * nothing and may be captured; only weights_create / _destroy / _status allocate or synchronise.  All pointers are memory of the
- * current device unless stated; strides count elements; an output must not overlap an input.  0 = accepted, -1 = refused before
+ * current device unless stated; strides count elements (at most 2^40); an output must not overlap an input.  0 = accepted, -1 = refused before
  * anything was launched.  One calling thread at a time; weights_create, _destroy and _status not while it captures. */
 #define SALT_B200_F32 0
 #define SALT_B200_BF16 1
@@ -606,8 +607,9 @@ int salt_b200_q4_expert_chain_static(const void *d_gate_vals, const void *d_gate
  * group_top (1 or 2) keys, the topk_groups best groups stay, and the topk (at most 32) best keys of their experts are selected;
  * the lowest index wins a tie.  weight = scale * score, divided by the sum of the selected scores if renormalize (a sum of zero
  * in double leaves zeros).  The bias never enters a weight.  The selection is that of 64-bit scores, whatever the type of the logits.
- * An expert whose logit or key is NaN or -infinity is never selected and takes no part in the softmax; logits of +infinity share
- * the whole softmax.  n_experts is at most 1024. */
+ * An expert whose logit is NaN or -infinity is never selected and takes no part in the softmax; one whose key is (by its bias) is
+ * never selected, but its score stays in the softmax.  Logits of +infinity share the whole softmax.  n_experts is at most 1024, scale
+ * finite. */
 typedef struct SaltB200RouteSpec {
     int n_experts, topk, scoring, n_groups, topk_groups, group_top, renormalize;
     float scale;
@@ -640,7 +642,7 @@ int salt_b200_mxfp4_quantize(const void *d_x, int dtype, size_t row_stride, int 
 #define SALT_B200_ACT_SILU 2
 /* Matrices [rows][cols] of n_experts experts (1: a dense projection).  Pointers are HOST or device memory; they are read on
  * `stream` before create returns and not kept: the handle holds its own copy, laid out once for the kernels in tiles of 128 rows and 256
- * columns (17 KB each; a gated pair's rows count together).  codes
+ * columns (17 KB each; a gated pair's rows count together).  rows is at most 2^24, n_experts 1024.  codes
  * [n_experts][rows][cols / 2], scales [n_experts][rows][cols / 32]; strides in bytes, 0 = dense.  With up_codes and up_scales (same
  * strides) the pair is gated: a product returns activation(gate row) * up row, and activation must be one of the two
  * functions.  A handle belongs to the device that is current when it is made; calls on another device are refused. */
@@ -665,7 +667,7 @@ int salt_b200_mxfp4_status(void *weights, void *stream);
 
 /* d_y[t] = sum over j of d_weights[t * topk + j] * d_rows[d_row_index[t * topk + j]], j ascending, in 32 bits, rounded once;
  * d_row_index NULL: row t * topk + j.  An index below zero or beyond n_rows adds nothing; a weight of zero still multiplies its row.
- * topk is at most 32.  Any alignment of whole elements. */
+ * topk is at most 32, cols 8388480, tokens * topk below 2^31.  Any alignment of whole elements. */
 int salt_b200_combine_experts(const void *d_rows, int dtype, size_t row_stride, int n_rows, int cols, const int32_t *d_row_index,
                               const float *d_weights, int tokens, int topk, void *d_y, int y_dtype, size_t y_row_stride,
                               void *stream);

@@ -24,7 +24,8 @@ int device_sms();
 // is a per-device attribute of the function; remembered per device and kernel, safe from any thread).
 cudaError_t ensure_dynamic_smem(const void* kernel, size_t bytes);
 // Dynamic shared memory of a launch that needs no such call: a block has 48 KB without one, and the kernel's static
-// variables (at most 6 KB in this library) count too.
+// variables count too.  They are at most 6 KB in the kernels that are launched by this rule; mxfp4_tensor_kernel has 9 KB and always
+// makes the call.
 constexpr size_t PLAIN_DYNAMIC_SMEM = 42 * 1024;
 
 // ---- q4_kernels.cu -------------------------------------------------------

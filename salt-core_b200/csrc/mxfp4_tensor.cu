@@ -7,7 +7,8 @@
 // unit belongs to is found in a prefix table over the groups' passes, made by every block from the device offsets.
 // Four launch forms, by a rule at the launch:
 //   passes of up to 96 rows: two blocks per SM, half of TMEM each; what bounds them is HBM (64 experts of 1536 x 5120, gate | up, 16 /
-//     31 / 63 rows each: 58 / 89 / 93 us, the last two 6.0 TB/s of 6.5 measured);
+//     31 / 63 rows in each of the 64, 541 to 558 MB: 85 / 89 / 92 us, 6.4 to 6.0 TB/s of 6.5 measured; by passes of up to 128 rows
+//     87 / 88 / 91);
 //   few units: a cluster of 2 to 8 blocks shares each, K split, and the partial sums meet in distributed shared memory; latency (one
 //     row of 4096 x 4096: 7.2 us);
 //   longer passes: a pair of SMs (cta_group::2) takes two row tiles of a pass and each loads half of its rows.  Loads from L2
@@ -21,7 +22,9 @@
 //   warp 8      issuer: tcgen05.cp of the chunk's scale tiles to TMEM, then its four MMAs; both run in issue order
 //   warps 4-7   epilogue: lane = weight row, column = row of the result; a gated pair's two rows are neighbouring lanes
 // Every mbarrier wait is bounded; on expiry the block raises its failure flag, sets SB_ERR_TIMEOUT, waits (bounded) for copies
-// and MMAs in flight, frees its TMEM and returns.
+// and MMAs in flight, frees its TMEM and returns.  The block's and the cluster's barriers have no limit of their own: every warp comes
+// to them, those that have given up as well.  Nor has the allocation of TMEM: what holds it does not wait for this block (see the
+// launch).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -7,12 +7,14 @@
 //   the lowest index among equals; w_e = scale * s_e, divided by the sum over the selected ones on request.
 //
 // A selection is a whole number, so it may not depend on how a sum was rounded.  Everything is computed in 32 bits first; where
-// the key (or the group score) that just won and the one that just lost are closer than the rounding errors of both, the
-// row is done again in 64 bits by the same code (about one row in a thousand of 256 experts with a bias).
+// the key that just won and the one that just lost, or the scores of a group that stays and of one that goes, are closer than the
+// rounding errors of both, and where a selected score is too small for 32 bits, the row is done again in 64 bits by the same code (of
+// rows of 256 experts one in 8500 with a bias, one in 1100 by groups of two keys without one).  Other weights are quotients of scores in
+// 32 bits: 5e-8 off on average, where rounding alone leaves 2e-8 to 3e-8.
 //
 // One warp per token: lane l holds experts l, l + 32, ...; the running maximum of the top-k is a warp-wide integer reduction of
 // order-preserving bit patterns.  Bound by the chain of reductions (two per selected expert), not by memory: 4099 tokens of 256
-// experts 8.1 us (plain softmax) and 14.6 us (sigmoid, bias, eight groups; 2 of them rows done again); grouping their 32 792 selections
+// experts 8.0 us (plain softmax) and 14.1 us (sigmoid, bias, eight groups; 1.2 of them a row done again); grouping their 32 792 selections
 // 7.5 us more, a dozen synchronised phases of one cluster.  One token of 128 experts, routed and grouped in one launch: 4 us.
 #include <cooperative_groups.h>
 #include <math_constants.h>
@@ -542,7 +544,7 @@ template <int VPT> cudaError_t launch_route(const RouteArgs& a, const GroupArgs*
         if (e != cudaSuccess) return e;
     }
     if (!g) return cudaSuccess;
-    const int warps = a.E <= 512 ? GR_WARPS : GR_WARPS / 2;          // two words per expert and warp: at most 139 KB
+    const int warps = a.E <= 512 ? GR_WARPS : GR_WARPS / 2;          // two words per expert and warp and three tables: at most 140 KB
     GroupArgs ga = *g;
     const int blocks = ga.n > GR_ONE_BLOCK ? GR_CLUSTER : 1;
     const long long held = (ga.n + (long long)warps * blocks - 1) / (warps * blocks);      // of a warp
