@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
             const bool live = m < a.w.stored_rows;
             // A store per row of the result writes 64 bytes a warp and takes some nine cycles of the SM; 16 bytes a lane, of rows that
             // lie together in shared memory, are four times less of them.
-            const bool stage_out = a.staged && m - q * 32 - lane + MX_TILE_ROWS <= a.w.stored_rows;
+            const bool stage_out = PAIR && a.staged && m - q * 32 - lane + MX_TILE_ROWS <= a.w.stored_rows;
             const uint32_t buf = done & 1u;
             ok = mbar_wait(&bar_done[buf], (done >> 1) & 1, fail);
             ok = __all_sync(0xffffffffu, ok);
@@ -523,10 +523,10 @@ __global__ void __launch_bounds__(MT_THREADS, 2) mxfp4_tensor_kernel(const MxTen
         }
         // Where results meet in shared memory a warp that has given up still comes to every barrier that the others may wait at, from
         // the unit that it broke off.  (Four warps that agree at a barrier with a reduction cost 2 us of 63.)
-        if (!ok && a.staged)
+        if (PAIR && !ok && a.staged)
             for (; u < units; u += unit_step) {
                 Unit un;
-                if (!groups.unit(u, &un) || ((PAIR ? 2 * un.tile + rank : un.tile) + 1) * MX_TILE_ROWS > a.w.stored_rows) continue;
+                if (!groups.unit(u, &un) || (2 * un.tile + rank + 1) * MX_TILE_ROWS > a.w.stored_rows) continue;
                 for (int n0 = 0; n0 < un.N; n0 += 32) {
                     epilogue_sync();
                     epilogue_sync();
@@ -637,9 +637,9 @@ cudaError_t launch_mxfp4_product(const Mxfp4Weights& w, const Mxfp4Call& c, cuda
     const bool pairs = small && (units * a.split > sms || a.share <= half);
     const bool pair = !small && a.split == 1 && w.row_tiles > 1;
     const size_t y_size = float_type_size(c.y_type);
-    // Results of long passes go through shared memory (4096 rows of 5120 x 5120: 48.5 -> 46.7 us); of short ones it costs what it
-    // saves (4096 of 5000 x 256: 17.6 and 19.0 us).
-    a.staged = !small && a.split == 1 && (uintptr_t)c.y % 16 == 0 && c.y_stride * y_size % 16 == 0;
+    // Results of pairs of SMs go through shared memory (4096 rows of 5120 x 5120: 48.5 -> 46.7 us); of short passes it costs what it
+    // saves (4096 of 5000 x 256: 17.6 and 19.0 us), and of single SMs too (18889 rows of 128 x 1408: 8.1 and 8.5).
+    a.staged = pair && (uintptr_t)c.y % 16 == 0 && c.y_stride * y_size % 16 == 0;
     const int slab = a.staged ? MT_BOX * MX_TILE_ROWS / (w.activation ? 2 : 1) * (int)y_size : 0;
     long long turns = 1;                                 // units of a block
     int grid = (int)units * a.split;

@@ -1,5 +1,5 @@
-"""Long passes whose results leave through shared memory: sixteen-byte rows of every type, full tiles beside a last one that is not,
-so that a block's epilogue takes both ways in turn; on pairs of SMs and on single ones."""
+"""Long passes with result rows on sixteen bytes, of every type: on pairs of SMs they leave through shared memory, full tiles beside a
+last one that is not, so that a block's epilogue takes both ways in turn; on single SMs they do not."""
 import numpy as np
 import pytest
 
